@@ -56,6 +56,7 @@ typedef struct fb200_device fb200_device;
 typedef struct fb200_qmatrix fb200_qmatrix;
 typedef struct fb200_kv_cache fb200_kv_cache;
 typedef struct fb200_llama fb200_llama;
+typedef struct fb200_f8matrix fb200_f8matrix;
 
 /* ---- device: fusor::Device::gpu(), fusor-ml/fusor/src/device.rs:29-40 -------------------------
  * One CUDA device + one stream per handle. `stream` may be an existing cudaStream_t (the
@@ -254,6 +255,44 @@ typedef struct fb200_sampler_config {
 FB200_API int fb200_sample(fb200_device* dev, const float* logits_dev, size_t rows, size_t n,
                            const fb200_sampler_config* cfg, const uint32_t* prev_dev, size_t prev_stride,
                            int prev_len, uint64_t counter, float* mu_dev, uint32_t* ids_dev);
+
+/* ---- 8-bit floats with a scale per block of 128 (no counterpart in the reference) ---------------------
+ * Linear layers of checkpoints whose weights are e4m3 codes with an f32 scale per block of 128 x 128, over activations that are quantised
+ * on the way in. A row of n values is n codes (one byte each) and ceil(n / 128) f32 scales; it stands for code x scale of its block.
+ * Blocks begin at columns 0, 128, ..; the last one may be shorter. Rows of codes lie `ld` bytes apart, ld >= n and a multiple of 16 like
+ * the address of the first; bytes n .. ld are neither read nor written. Scales are contiguous, [rows, ceil(n / 128)].
+ * Quantisation: a = the largest magnitude of the block, at least 7 x 2^-120; scale = a / 448, code = e4m3(v x (448 / a)) rounded to
+ * nearest even, both quotients in f32. A block with an infinity or a NaN gets NaN for its scale and all its codes.
+ * Inputs are F32, F16 or BF16 (`type`), rows `ldx` .. elements apart; arithmetic is f32. Outputs may not overlap inputs, unless said so.
+ * FB200_ERR_UNSUPPORTED_DTYPE for other types, FB200_ERR_INVALID_SHAPE for rows that overlap or are not aligned, for 2^31 rows or more
+ * and for more than 2^27 columns. Zero rows or columns: nothing is written. */
+FB200_API int fb200_quantize_f8(fb200_device* dev, const void* x_dev, size_t ldx, uint32_t type, size_t rows, size_t n, uint8_t* codes_dev,
+                                size_t ld, float* scales_dev);
+/* The same of silu(gate) * up, the hidden row of a gated feed-forward (gate and up may be halves of the same rows). */
+FB200_API int fb200_silu_mul_f8(fb200_device* dev, const void* gate_dev, size_t ldgate, const void* up_dev, size_t ldup, uint32_t type,
+                                size_t rows, size_t n, uint8_t* codes_dev, size_t ld, float* scales_dev);
+/* The same of an RMSNorm: s = x (+ residual), v = s / sqrt(mean(s^2) + eps) * weight (+ bias), weight and bias f32 [n]. residual_dev,
+ * bias_dev and sum_dev may be NULL; sum_dev receives s rounded to `type` (the norm is of s before that rounding) and may be x_dev or
+ * residual_dev themselves, at the same distance of rows. n <= 32768 (FB200_ERR_INVALID_SHAPE). */
+FB200_API int fb200_rms_norm_f8(fb200_device* dev, const void* x_dev, size_t ldx, const void* residual_dev, size_t ldres, void* sum_dev,
+                                size_t ldsum, uint32_t type, const float* weight_dev, const float* bias_dev, float eps, size_t rows,
+                                size_t n, uint8_t* codes_dev, size_t ld, float* scales_dev);
+/* A weight matrix [N, K] of codes with scales [ceil(N / 128), ceil(K / 128)]. from_raw_bytes copies N x K codes and the scales from the
+ * host. from_device takes device buffers as they are (rows of codes ld bytes apart, as above), waits for the stream, and reads them in
+ * every product: they have to outlive the handle and may not change while it lives (products fetch them ahead of the kernels in front).
+ * N and K from 1 to 2^27. */
+FB200_API int fb200_f8matrix_from_raw_bytes(fb200_device* dev, const uint64_t* shape, int rank, const void* codes_host, size_t nbytes,
+                                            const float* scales_host, size_t nscales, fb200_f8matrix** out);
+FB200_API int fb200_f8matrix_from_device(fb200_device* dev, const uint64_t* shape, int rank, const uint8_t* codes_dev, size_t ld,
+                                         const float* scales_dev, fb200_f8matrix** out);
+FB200_API int fb200_f8matrix_free(fb200_f8matrix* w);
+FB200_API int fb200_f8matrix_shape(const fb200_f8matrix* w, uint64_t* n_out, uint64_t* k_out);
+/* y[M, N] = x[M, K] . W^T (+ epilogue), y contiguous, F32, F16 or BF16 (`y_type`), rounded once. x is M rows of K codes and their scales.
+ * The products of a block of 128 are summed by the tensor cores, the blocks under (x scale) x (W scale) in f32. Epilogues:
+ * FB200_EPI_RESIDUAL and FB200_EPI_BIAS as in fb200_q_mat_mul (r1, r2 f32; an f32 y may be r1 or r2); no FB200_EPI_SWIGLU
+ * (FB200_ERR_UNSUPPORTED_DTYPE). Results do not depend on timing; they may differ in the last bits between numbers of rows. */
+FB200_API int fb200_f8_mat_mul(fb200_device* dev, const uint8_t* codes_dev, size_t ld, const float* scales_dev, size_t m,
+                               const fb200_f8matrix* w, uint32_t y_type, void* y_dev, const fb200_epilogue* epilogue);
 
 /* ---- KV cache: KvCache / TensorCache, fusor-ml/fusor/src/cache/kv_cache.rs:12-68 ----------------
  * Layout [B, Hkv, capacity, D], fp16 on the device (the reference's cache is f32). Capacity

@@ -114,6 +114,8 @@ EXPORTS = [
     "fb200_llama_create_layers", "fb200_llama_logits_at",
     "fb200_comm_unique_id", "fb200_comm_create", "fb200_comm_destroy", "fb200_comm_all_reduce_sum",
     "fb200_comm_exchange_handle", "fb200_comm_exchange_attach", "fb200_exchange_wait_check",
+    "fb200_quantize_f8", "fb200_silu_mul_f8", "fb200_rms_norm_f8", "fb200_f8matrix_from_raw_bytes", "fb200_f8matrix_from_device",
+    "fb200_f8matrix_free", "fb200_f8matrix_shape", "fb200_f8_mat_mul",
 ]
 
 _lib = None
@@ -194,6 +196,14 @@ def load_library():
         "fb200_comm_exchange_handle": (i32, [vp, sz, vp, sz]),
         "fb200_comm_exchange_attach": (i32, [vp, vp, sz]),
         "fb200_exchange_wait_check": (i32, [vp, i32]),
+        "fb200_quantize_f8": (i32, [vp, vp, sz, u32, sz, sz, vp, sz, vp]),
+        "fb200_silu_mul_f8": (i32, [vp, vp, sz, vp, sz, u32, sz, sz, vp, sz, vp]),
+        "fb200_rms_norm_f8": (i32, [vp, vp, sz, vp, sz, vp, sz, u32, vp, vp, f32, sz, sz, vp, sz, vp]),
+        "fb200_f8matrix_from_raw_bytes": (i32, [vp, C.POINTER(u64), i32, vp, sz, vp, sz, pp]),
+        "fb200_f8matrix_from_device": (i32, [vp, C.POINTER(u64), i32, vp, sz, vp, pp]),
+        "fb200_f8matrix_free": (i32, [vp]),
+        "fb200_f8matrix_shape": (i32, [vp, C.POINTER(u64), C.POINTER(u64)]),
+        "fb200_f8_mat_mul": (i32, [vp, vp, sz, vp, sz, vp, u32, vp, C.POINTER(_Epilogue)]),
     }
     for name, (res, args) in sig.items():
         if LIB_PATH.endswith("_dense.so") and not hasattr(L, name):
@@ -416,6 +426,48 @@ class Device:
                                                    mask_kind, out.ptr))
         return out
 
+    # ---- rows of 8-bit floats ------------------------------------------------------------
+    def quantize_f8(self, x: Tensor, out: "F8Rows" = None) -> "F8Rows":
+        """Rows of x (f32, f16, or bf16 as uint16) as e4m3 codes with a scale per block of 128 columns."""
+        kind, rows, n = _f8_input(self, "x", x)
+        out = _f8_output(self, out, x.shape)
+        self._check(self.lib.fb200_quantize_f8(self.h, x.ptr, n, kind, rows, n, out.codes.ptr, out.ld, out.scales.ptr))
+        return out
+
+    def silu_mul_f8(self, gate: Tensor, up: Tensor = None, out: "F8Rows" = None) -> "F8Rows":
+        """silu(gate) * up as rows of 8 bits. Without `up` the rows of `gate` are [gate | up], as one stacked product leaves them."""
+        kind, rows, n = _f8_input(self, "gate", gate)
+        ld, shape, gp = n, gate.shape, gate.ptr
+        if up is None:
+            if n % 2:
+                raise FusorError(ERR_INVALID_SHAPE, f"rows of {n} values have no halves")
+            n //= 2
+            shape, upp = shape[:-1] + (n,), gp + n * gate.dtype.itemsize
+        else:
+            if up.shape != gate.shape or up.dtype != gate.dtype or up.device is not self:
+                raise FusorError(ERR_INVALID_SHAPE, "up must be a tensor like gate")
+            upp = up.ptr
+        out = _f8_output(self, out, shape)
+        self._check(self.lib.fb200_silu_mul_f8(self.h, gp, ld, upp, ld, kind, rows, n, out.codes.ptr, out.ld, out.scales.ptr))
+        return out
+
+    def rms_norm_f8(self, x: Tensor, weight: Tensor, eps: float, residual: Tensor = None, bias: Tensor = None,
+                    sum_out: Tensor = None, out: "F8Rows" = None) -> "F8Rows":
+        """RMSNorm of x (+ residual) as rows of 8 bits; `sum_out` receives x + residual and may be x or residual itself."""
+        kind, rows, n = _f8_input(self, "x", x)
+        for name, t in (("residual", residual), ("sum_out", sum_out)):
+            if t is not None and (t.nbytes != x.nbytes or t.dtype != x.dtype or t.device is not self):
+                raise FusorError(ERR_INVALID_SHAPE, f"{name} must be a tensor like x")
+        x._require_f32("weight", weight, n)
+        x._require_f32("bias", bias, n)
+        out = _f8_output(self, out, x.shape)
+        self._check(self.lib.fb200_rms_norm_f8(self.h, x.ptr, n, residual.ptr if residual is not None else None, n,
+                                               sum_out.ptr if sum_out is not None else None, n, kind,
+                                               weight.ptr if weight is not None else None,
+                                               bias.ptr if bias is not None else None, eps, rows, n, out.codes.ptr, out.ld,
+                                               out.scales.ptr))
+        return out
+
     def close(self) -> None:
         if self.h:
             self.lib.fb200_device_destroy(self.h)
@@ -486,6 +538,141 @@ class QMatrix:
     def free(self) -> None:
         if self.h:
             self.device.lib.fb200_qmatrix_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+# element types of rows that become 8-bit floats, and of products over them; bf16 values travel as their bits
+_F8_TYPES = {np.dtype(np.float32): F32, np.dtype(np.float16): F16, np.dtype(np.uint16): BF16}
+_F8_OUT = {F32: np.dtype(np.float32), F16: np.dtype(np.float16), BF16: np.dtype(np.uint16)}
+
+
+def _f8_input(device: Device, name: str, x: Tensor):
+    """(type, rows, columns) of a tensor whose last axis becomes rows of 8 bits."""
+    kind = _F8_TYPES.get(x.dtype)
+    if kind is None or not x.shape or x.device is not device:
+        raise FusorError(ERR_UNSUPPORTED_DTYPE, f"{name} must be an f32, f16 or bf16 (uint16) tensor with rows on this device handle "
+                                                f"(got {x.dtype}, shape {x.shape})")
+    n = x.shape[-1]
+    return kind, (x.nbytes // x.dtype.itemsize // n if n else 0), n
+
+
+def _f8_output(device: Device, out: Optional["F8Rows"], shape) -> "F8Rows":
+    if out is None:
+        return F8Rows(device, shape)
+    if out.shape[-1:] != shape[-1:] or out.rows != _rows_of(shape) or out.device is not device:
+        raise FusorError(ERR_INVALID_SHAPE, f"out must hold rows of shape {tuple(shape)} on this device handle (got {out.shape})")
+    return out
+
+
+def _rows_of(shape) -> int:
+    rows = 1
+    for s in shape[:-1]:
+        rows *= s
+    return rows
+
+
+def _f8_values(codes: np.ndarray) -> np.ndarray:
+    """f32 values of e4m3 codes."""
+    b = np.arange(256)
+    e, f = (b >> 3) & 15, b & 7
+    table = np.where(e > 0, np.ldexp(8.0 + f, e - 10), np.ldexp(1.0 * f, -9)).astype(np.float32)
+    table[(b & 127) == 127] = np.nan
+    return (table * np.where(b > 127, np.float32(-1), np.float32(1)))[codes]
+
+
+class F8Rows:
+    """Rows of e4m3 codes with an f32 scale per block of 128 columns. `codes` is a uint8 tensor [rows, ld] (ld a multiple of 16),
+    `scales` an f32 tensor [rows, ceil(n / 128)]; both are made here or the caller's."""
+
+    def __init__(self, device: Device, shape: Sequence[int], codes: Tensor = None, scales: Tensor = None):
+        self.device, self.shape = device, tuple(int(s) for s in shape)
+        self.rows, n = _rows_of(self.shape), self.shape[-1]
+        self.blocks = -(-n // 128)
+        self.codes = Tensor(device, (self.rows, -(-n // 16) * 16), np.uint8) if codes is None else codes
+        self.scales = Tensor(device, (self.rows, self.blocks), np.float32) if scales is None else scales
+        self.ld = self.codes.shape[-1]
+        if (self.codes.dtype != np.uint8 or self.codes.shape[:-1] != (self.rows,) or self.ld < n or self.ld % 16 or
+                self.codes.device is not device):
+            raise FusorError(ERR_INVALID_SHAPE, f"codes must be uint8 [{self.rows}, a multiple of 16 from {n} on] (got {self.codes.dtype} "
+                                                f"{self.codes.shape})")
+        if self.scales.dtype != np.float32 or self.scales.shape != (self.rows, self.blocks) or self.scales.device is not device:
+            raise FusorError(ERR_INVALID_SHAPE, f"scales must be float32 [{self.rows}, {self.blocks}] (got {self.scales.dtype} "
+                                                f"{self.scales.shape})")
+
+    def as_slice(self) -> np.ndarray:
+        """The values that the rows stand for, read back as f32."""
+        n = self.shape[-1]
+        scales = np.repeat(self.scales.as_slice(), 128, axis=1)[:, :n]
+        return (_f8_values(self.codes.as_slice()[:, :n]) * scales).reshape(self.shape)
+
+    def f8_mat_mul(self, w: "F8Matrix", out_type: int = F32, epilogue: int = EPI_NONE, r1: Tensor = None, r2: Tensor = None,
+                   out: Tensor = None) -> Tensor:
+        """self [.., K] . W[N, K]^T (+ residuals or bias, f32) as F32, F16 or BF16 (a uint16 tensor of their bits)."""
+        n, k = w.shape
+        if self.shape[-1] != k:
+            raise FusorError(ERR_INVALID_SHAPE, f"lhs columns ({self.shape[-1]}) != weight in_features ({k})")
+        kind = _F8_OUT.get(out_type)
+        if kind is None:
+            raise FusorError(ERR_UNSUPPORTED_DTYPE, f"outputs are F32, F16 or BF16 (got type {out_type})")
+        d, m = self.device, self.rows
+        if out is None:
+            out = Tensor(d, self.shape[:-1] + (n,), kind)
+        elif out.dtype != kind or out.nbytes < m * n * kind.itemsize or out.device is not d:
+            raise FusorError(ERR_INVALID_SHAPE, f"out must be a {kind} tensor of at least {m * n} elements on the same device handle "
+                                                f"(got {out.dtype}, {out.nbytes} bytes)")
+        self.codes._require_f32("r1", r1, n if epilogue == EPI_BIAS else m * n)
+        self.codes._require_f32("r2", r2, m * n)
+        ep = _Epilogue(epilogue, r1.ptr if r1 is not None else None, r2.ptr if r2 is not None else None)
+        d._check(d.lib.fb200_f8_mat_mul(d.h, self.codes.ptr, self.ld, self.scales.ptr, m, w.h, out_type, out.ptr, C.byref(ep)))
+        return out
+
+
+class F8Matrix:
+    """A weight matrix [N, K] of e4m3 codes with an f32 scale per block of 128 x 128."""
+
+    def __init__(self, device: Device, handle: int, held=()):
+        self.device, self.h, self._held = device, handle, held
+        n, k = C.c_uint64(), C.c_uint64()
+        device.lib.fb200_f8matrix_shape(handle, C.byref(n), C.byref(k))
+        self.shape = (n.value, k.value)
+
+    @classmethod
+    def from_raw_bytes(cls, device: Device, shape: Sequence[int], codes, scales) -> "F8Matrix":
+        """Copies N x K codes (bytes) and [ceil(N / 128), ceil(K / 128)] f32 scales to the device."""
+        codes = np.ascontiguousarray(codes).view(np.uint8).reshape(-1)
+        scales = np.ascontiguousarray(scales, dtype=np.float32).reshape(-1)
+        shp = (C.c_uint64 * len(shape))(*[int(s) for s in shape])
+        out = C.c_void_p()
+        device._check(device.lib.fb200_f8matrix_from_raw_bytes(device.h, shp, len(shape), _hp(codes), codes.size, _hp(scales),
+                                                               scales.size, C.byref(out)))
+        return cls(device, out.value)
+
+    @classmethod
+    def from_tensors(cls, codes: Tensor, scales: Tensor, k: int = None) -> "F8Matrix":
+        """A matrix over device tensors as they are: uint8 [N, ld], of which the first k columns count (all without k), and f32
+        [ceil(N / 128), ceil(k / 128)]. Their contents may not change while the matrix lives."""
+        device = codes.device
+        if codes.dtype != np.uint8 or len(codes.shape) != 2:
+            raise FusorError(ERR_INVALID_SHAPE, f"codes must be a uint8 tensor [N, ld] (got {codes.dtype} {codes.shape})")
+        n, ld = codes.shape
+        k = ld if k is None else int(k)
+        if not 0 < k <= ld or scales.dtype != np.float32 or scales.shape != (-(-n // 128), -(-k // 128)) or scales.device is not device:
+            raise FusorError(ERR_INVALID_SHAPE, f"scales must be float32 [{-(-n // 128)}, {-(-k // 128)}] for {k} of {ld} columns (got "
+                                                f"{scales.dtype} {scales.shape})")
+        shp = (C.c_uint64 * 2)(n, k)
+        out = C.c_void_p()
+        device._check(device.lib.fb200_f8matrix_from_device(device.h, shp, 2, codes.ptr, ld, scales.ptr, C.byref(out)))
+        return cls(device, out.value, (codes, scales))
+
+    def free(self) -> None:
+        if self.h:
+            self.device.lib.fb200_f8matrix_free(self.h)
             self.h = None
 
     def __del__(self):

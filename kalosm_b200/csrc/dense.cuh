@@ -70,3 +70,5 @@ __device__ __forceinline__ float fb_gelu_tanh_fast(float v) {
 struct CUtensorMap_st;
 bool fb200_make_map_2d(CUtensorMap_st* map, const void* base, int bf16, uint64_t cols, uint64_t rows, uint64_t row_stride_bytes,
                        uint32_t box_rows);
+// The same of bytes, boxes of 128 columns x box_rows rows
+bool fb200_make_map_2d_bytes(CUtensorMap_st* map, const void* base, uint64_t cols, uint64_t rows, uint64_t row_stride_bytes, uint32_t box_rows);

@@ -228,8 +228,8 @@ int launch_tc(fb200_device* dev, const fb200_dense_job& j, DenseTcArgs a) {
 
 }  // namespace
 
-bool fb200_make_map_2d(CUtensorMap_st* map, const void* base, int bf16, uint64_t cols, uint64_t rows, uint64_t row_stride_bytes,
-                       uint32_t box_rows) {
+// The driver's encoder, looked up once
+static encode_fn tensor_map_encoder() {
   static encode_fn enc = [] {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -237,12 +237,26 @@ bool fb200_make_map_2d(CUtensorMap_st* map, const void* base, int bf16, uint64_t
       p = nullptr;
     return reinterpret_cast<encode_fn>(p);
   }();
+  return enc;
+}
+
+static bool make_map(CUtensorMap_st* map, CUtensorMapDataType type, uint32_t box_cols, const void* base, uint64_t cols, uint64_t rows,
+                     uint64_t row_stride_bytes, uint32_t box_rows) {
+  const encode_fn enc = tensor_map_encoder();
   if (!enc) return false;
   const cuuint64_t dims[2] = {cols, rows}, strides[1] = {row_stride_bytes};
-  const cuuint32_t box[2] = {64, box_rows}, estr[2] = {1, 1};
-  return enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box,
-             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const cuuint32_t box[2] = {box_cols, box_rows}, estr[2] = {1, 1};
+  return enc(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool fb200_make_map_2d(CUtensorMap_st* map, const void* base, int bf16, uint64_t cols, uint64_t rows, uint64_t row_stride_bytes,
+                       uint32_t box_rows) {
+  return make_map(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 64, base, cols, rows, row_stride_bytes, box_rows);
+}
+
+bool fb200_make_map_2d_bytes(CUtensorMap_st* map, const void* base, uint64_t cols, uint64_t rows, uint64_t row_stride_bytes, uint32_t box_rows) {
+  return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 128, base, cols, rows, row_stride_bytes, box_rows);
 }
 
 int fb200_dense_gemm_tc(fb200_device* dev, const fb200_dense_job& j) {

@@ -1,0 +1,675 @@
+// Products of 8-bit floats: rows of e4m3 codes with an f32 scale per block of 128 columns, times a matrix of e4m3 codes with an f32
+// scale per block of 128 x 128.
+//
+//   y[m, n] = sum over blocks b of 128 columns of  sx[m, b] sw[n / 128, b] * (sum over k in b of x[m, k] w[n, k])   (+ residual or bias)
+//
+// The inner sum is one accumulation of the tensor cores (tcgen05.mma kind::f8f6f4, f32 in tensor memory): a block of 128 codes is exactly
+// one row of a 128-byte swizzled operand and four MMAs. The outer sum is kept in f32 registers: the epilogue warps take each block's
+// accumulator out of tensor memory while the tensor cores fill the next one, and add it under its scale.
+//
+// f8_few_kernel (weights in the M role): 128 weight rows by BM activation rows per CTA, K split over a cluster whose CTAs join their sums
+// through distributed shared memory in the order of their ranks. Bound: HBM (N K bytes) for few rows.
+// f8_pair_kernel (activations in the M role): CTA pairs, 256 activation rows by NW weight rows. Bound: tensor cores.
+// Every wait is bounded (2^22 polls): one that gives up sets the device status word and a flag that makes the other roles leave; copies
+// and MMAs in flight are waited for, TMEM is released on every path.
+#include <cstdlib>
+#include <new>
+
+#include "dense.cuh"
+#include "state_columns.cuh"
+#include "tcgen05.cuh"
+
+// A matrix [n, k] of codes, `ld` bytes from row to row, and its scales [ceil(n / 128), ceil(k / 128)]
+struct fb200_f8matrix {
+  fb200_device* dev = nullptr;
+  uint64_t n = 0, k = 0;
+  size_t ld = 0;
+  uint8_t* codes = nullptr;
+  float* scales = nullptr;
+  bool owned = false;
+  CUtensorMap map128, map64;  // boxes of 128 and of 64 rows
+};
+
+namespace {
+
+constexpr int F8_BLOCK = 128, F8_A_BYTES = 128 * 128;
+
+struct F8Out {
+  void* y;
+  uint32_t type;
+  const float *r1, *r2, *bias;
+  int m, n;
+};
+
+__device__ __forceinline__ float f8_epilogue(const F8Out& o, float v, int m, int n) {
+  const size_t at = (size_t)m * o.n + n;
+  if (o.bias) v += o.bias[n];
+  if (o.r1) v += o.r1[at];
+  if (o.r2) v += o.r2[at];
+  return v;
+}
+__device__ __forceinline__ void f8_put(const F8Out& o, float v, int m, int n) {
+  const size_t at = (size_t)m * o.n + n;
+  v = f8_epilogue(o, v, m, n);
+  if (o.type == FB200_F32) reinterpret_cast<float*>(o.y)[at] = v;
+  else if (o.type == FB200_BF16) reinterpret_cast<__nv_bfloat16*>(o.y)[at] = __float2bfloat16(v);
+  else reinterpret_cast<__half*>(o.y)[at] = __float2half(v);
+}
+
+// ---- few activation rows ------------------------------------------------------------------------------------------------
+
+constexpr int FEW_SCALES = 16;  // blocks of K whose scales are fetched together
+
+template <int BM>
+struct Few {
+  static constexpr int EPI_WARPS = BM >= 64 ? 8 : 4, THREADS = (EPI_WARPS + 2) * 32;
+  static constexpr int COLS = BM * 4 / EPI_WARPS;  // activation rows of an epilogue thread
+  static constexpr int STAGE = F8_A_BYTES + BM * 128;
+  static constexpr int STAGES = BM == 16 ? 6 : BM == 32 ? 5 : BM == 64 ? 4 : 6;
+  static constexpr int BUFS = 4, TMEM = BUFS * BM;
+  static constexpr int SCALE_ROW = BM + 4, SCALE_BYTES = 2 * FEW_SCALES * SCALE_ROW * 4;
+  static constexpr int SMEM = STAGES * STAGE + SCALE_BYTES + 256 + 1024;
+  static constexpr int PER_SM = BM <= 64 ? 2 : 1;
+  // instruction descriptor: f32 accumulator, e4m3 A and B, both K-major, N = BM, M = 128
+  static constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(BM >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+  static_assert(STAGES * STAGE >= BM * 128 * 4, "the partial sums take the operands' place");
+};
+
+struct FewArgs {
+  const float *sx, *sw;
+  F8Out out;
+  int kblocks, m_tiles, split;
+  int* status;
+};
+
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int BM>
+__global__ void __launch_bounds__(Few<BM>::THREADS, Few<BM>::PER_SM)
+f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
+  using F = Few<BM>;
+  extern __shared__ uint8_t sm_raw[];
+  // the same offset in every CTA of the cluster: their dynamic shared memory starts at the same address
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~(uintptr_t)1023);
+  float* scales = reinterpret_cast<float*>(sm + F::STAGES * F::STAGE);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + F::STAGES * F::STAGE + F::SCALE_BYTES);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * F::STAGES + 2 * F::BUFS + 1);
+  volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const uint32_t full = smem_u32(bars), stage_free = full + 8 * F::STAGES, acc_full = stage_free + 8 * F::STAGES, acc_free = acc_full + 8 * F::BUFS,
+                 drained = acc_free + 8 * F::BUFS;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = (int)cluster_rank(), tile = (int)blockIdx.x / a.split;
+  // activation tiles fastest: the CTAs that run together share their weight rows in L2
+  const int nt = tile / a.m_tiles, mt = tile - nt * a.m_tiles, m0 = mt * BM;
+  const int kb0 = (int)((long long)a.kblocks * rank / a.split), nkb = (int)((long long)a.kblocks * (rank + 1) / a.split) - kb0;
+
+  if (tid == 0) {
+    *dead = 0;
+    for (int i = 0; i < F::STAGES; ++i) { mbar_init(full + 8 * i, 1); mbar_init(stage_free + 8 * i, 1); }
+    for (int i = 0; i < F::BUFS; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_free + 8 * i, F::EPI_WARPS); }
+    mbar_init(drained, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(F::TMEM) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents_small();  // behind the allocation: a dependent must not take columns that this grid still waits for
+
+  float2 acc[F::COLS / 2];
+#pragma unroll
+  for (int i = 0; i < F::COLS / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+
+  if (warp < F::EPI_WARPS) {
+    // ---- epilogue: warp w reads TMEM lanes 32 (w % 4) .. = weight rows, COLS of the activation rows
+    const int quad = warp & 3, col0 = (warp >> 2) * F::COLS;
+    constexpr int ET = F::EPI_WARPS * 32, MINE = FEW_SCALES * BM / ET;
+    float ahead[MINE];
+    // scales of FEW_SCALES blocks: thread t holds block t % 16 of activation rows t / 16, ..
+    auto fetch = [&](int first) {
+      const int kb = kb0 + first + (tid % FEW_SCALES);
+      const bool in = first + (tid % FEW_SCALES) < nkb;
+      const float w = in ? a.sw[(size_t)nt * a.kblocks + kb] : 0.f;
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
+        const int m = m0 + tid / FEW_SCALES + i * (ET / FEW_SCALES);
+        ahead[i] = in && m < a.out.m ? a.sx[(size_t)m * a.kblocks + kb] * w : 0.f;
+      }
+    };
+    pdl_wait();
+    fetch(0);
+    for (int i = 0; i < nkb; ++i) {
+      const int buf = i % F::BUFS, at = i % FEW_SCALES;
+      if (at == 0) {
+        // the other half was last read before everybody came to this barrier's predecessor
+        float* half = scales + ((i / FEW_SCALES) & 1) * FEW_SCALES * F::SCALE_ROW;
+#pragma unroll
+        for (int j = 0; j < MINE; ++j) half[(tid % FEW_SCALES) * F::SCALE_ROW + tid / FEW_SCALES + j * (ET / FEW_SCALES)] = ahead[j];
+        asm volatile("bar.sync 1, %0;" ::"n"(ET) : "memory");
+        if (i + FEW_SCALES < nkb) fetch(i + FEW_SCALES);
+      }
+      if (!w_wait(acc_full + 8 * buf, (uint32_t)((i / F::BUFS) & 1), dead, a.status)) {
+        // the barriers of the scales to come are met all the same
+        for (int j = (i / FEW_SCALES + 1) * FEW_SCALES; j < nkb; j += FEW_SCALES) asm volatile("bar.sync 1, %0;" ::"n"(ET) : "memory");
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t tl = tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(buf * BM + col0);
+      uint32_t v[F::COLS / 16][16];
+#pragma unroll
+      for (int j = 0; j < F::COLS / 16; ++j) x_ld16(tl + 16 * j, v[j]);
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_free + 8 * buf);
+      const float4* sc = reinterpret_cast<const float4*>(scales + (((i / FEW_SCALES) & 1) * FEW_SCALES + at) * F::SCALE_ROW + col0);
+#pragma unroll
+      for (int j = 0; j < F::COLS / 4; ++j) {
+        const float4 s = sc[j];
+        const uint32_t* p = &v[j / 4][4 * (j % 4)];
+        acc[2 * j] = fma2(make_float2(__uint_as_float(p[0]), __uint_as_float(p[1])), make_float2(s.x, s.y), acc[2 * j]);
+        acc[2 * j + 1] = fma2(make_float2(__uint_as_float(p[2]), __uint_as_float(p[3])), make_float2(s.z, s.w), acc[2 * j + 1]);
+      }
+    }
+  } else if (warp == F::EPI_WARPS) {
+    // ---- copy requester; the weights do not depend on the kernel in front
+    if (lane == 0) {
+      const int pre = min(F::STAGES, nkb);
+      for (int i = 0; i < pre; ++i) {
+        mbar_expect_tx(full + 8 * i, F::STAGE);
+        x_tma_box2(smem_u32(sm + i * F::STAGE), &wmap, (kb0 + i) * F8_BLOCK, nt * 128, full + 8 * i);
+      }
+      pdl_wait();
+      int i = 0;
+      for (; i < pre; ++i) x_tma_box2(smem_u32(sm + i * F::STAGE + F8_A_BYTES), &xmap, (kb0 + i) * F8_BLOCK, m0, full + 8 * i);
+      for (; i < nkb; ++i) {
+        const int s = i % F::STAGES;
+        if (!x_wait(stage_free + 8 * s, (uint32_t)((i / F::STAGES - 1) & 1), dead, a.status)) break;
+        const uint32_t dst = smem_u32(sm + s * F::STAGE), bar = full + 8 * s;
+        mbar_expect_tx(bar, F::STAGE);
+        x_tma_box2(dst, &wmap, (kb0 + i) * F8_BLOCK, nt * 128, bar);
+        x_tma_box2(dst + F8_A_BYTES, &xmap, (kb0 + i) * F8_BLOCK, m0, bar);
+      }
+      if (*dead)
+        for (int j = max(0, i - F::STAGES); j < i; ++j) x_drain(full + 8 * (j % F::STAGES), (uint32_t)((j / F::STAGES) & 1));
+    }
+  } else {
+    // ---- MMA issuer
+    const uint64_t adesc0 = x_desc_rows(smem_u32(sm)), bdesc0 = x_desc_rows(smem_u32(sm) + F8_A_BYTES);
+    bool alive = true;
+    for (int i = 0; i < nkb && alive; ++i) {
+      const int s = i % F::STAGES, buf = i % F::BUFS;
+      if (i >= F::BUFS && !(alive = w_wait(acc_free + 8 * buf, (uint32_t)((i / F::BUFS - 1) & 1), dead, a.status))) break;
+      if (!(alive = w_wait(full + 8 * s, (uint32_t)((i / F::STAGES) & 1), dead, a.status))) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint64_t at = (uint64_t)((s * F::STAGE) >> 4);
+      w_mma4_f8<2, 2>(tmem + (uint32_t)(buf * BM), adesc0 + at, bdesc0 + at, F::IDESC, 0u);
+      w_commit(stage_free + 8 * s);
+      w_commit(acc_full + 8 * buf);
+    }
+    w_commit(drained);
+    x_drain(drained, 0);
+  }
+  __syncwarp();
+
+  // ---- the sums of the cluster's ranges of K, joined in the order of the ranks
+  const int quad = warp & 3, col0 = (warp >> 2) * F::COLS, n = nt * 128 + 32 * quad + lane;
+  if (a.split == 1) {
+    if (warp < F::EPI_WARPS && n < a.out.n)
+#pragma unroll
+      for (int j = 0; j < F::COLS; ++j)
+        if (m0 + col0 + j < a.out.m) f8_put(a.out, j & 1 ? acc[j / 2].y : acc[j / 2].x, m0 + col0 + j, n);
+  } else {
+    __syncthreads();  // nobody multiplies from the operands any more
+    float* part = reinterpret_cast<float*>(sm);
+    if (warp < F::EPI_WARPS)
+#pragma unroll
+      for (int j = 0; j < F::COLS; ++j) part[(col0 + j) * 128 + 32 * quad + lane] = j & 1 ? acc[j / 2].y : acc[j / 2].x;
+    cluster_sync();
+    if (warp < F::EPI_WARPS && n < a.out.n) {
+      const int per = BM / a.split;
+      for (int j = rank * per + (warp >> 2); j < (rank + 1) * per && m0 + j < a.out.m; j += F::EPI_WARPS / 4) {
+        const uint32_t mine = smem_u32(part + j * 128 + 32 * quad + lane);
+        float v = 0.f;
+        for (int q = 0; q < a.split; ++q) v += ld_cluster(cluster_addr(mine, (uint32_t)q));
+        f8_put(a.out, v, m0 + j, n);
+      }
+    }
+    cluster_sync();  // the others may still read
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(F::TMEM) : "memory");
+}
+
+// ---- many activation rows -----------------------------------------------------------------------------------------------
+
+constexpr int PAIR_EPI_WARPS = 8, PAIR_THREADS = (PAIR_EPI_WARPS + 2) * 32, PAIR_MAX_STAGES = 8;
+constexpr int TURN_ROW = 20, TURN_BYTES = 32 * TURN_ROW * 4;  // a warp's 32 rows x 16 columns on their way out, rows 80 bytes apart
+
+template <int NW>
+struct Pair {
+  static constexpr int STAGE = F8_A_BYTES + NW / 2 * 128, STAGES = NW == 256 ? 6 : 8, TMEM = 2 * NW;
+  static constexpr int SMEM = STAGES * STAGE + PAIR_EPI_WARPS * TURN_BYTES + 256 + 1024;
+  // instruction descriptor: f32 accumulator, e4m3 A and B, both K-major, N = NW, M = 256 over the pair
+  static constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(NW >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+};
+
+struct PairArgs {
+  const float *sx, *sw;
+  F8Out out;
+  int kblocks, m_tiles, n_tiles, m_group;
+  int vec;  // four columns of y (and of the residuals) are aligned
+  int* status;
+};
+
+// Four neighbouring outputs
+__device__ __forceinline__ void f8_put4(const F8Out& o, float4 v, int m, int n) {
+  const size_t at = (size_t)m * o.n + n;
+  if (o.bias) { v.x += o.bias[n]; v.y += o.bias[n + 1]; v.z += o.bias[n + 2]; v.w += o.bias[n + 3]; }
+  if (o.r1) { const float4 r = *reinterpret_cast<const float4*>(o.r1 + at); v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w; }
+  if (o.r2) { const float4 r = *reinterpret_cast<const float4*>(o.r2 + at); v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w; }
+  if (o.type == FB200_F32) {
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(o.y) + at) = v;
+  } else if (o.type == FB200_BF16) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(v.x, v.y), q = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(o.y) + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&p), *reinterpret_cast<const uint32_t*>(&q));
+  } else {
+    const __half2 p = __floats2half2_rn(v.x, v.y), q = __floats2half2_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(o.y) + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&p), *reinterpret_cast<const uint32_t*>(&q));
+  }
+}
+
+template <int NW>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
+  using P = Pair<NW>;
+  extern __shared__ uint8_t sm_raw[];
+  // the same offset in both CTAs: their dynamic shared memory starts at the same address
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~(uintptr_t)1023);
+  float* turn = reinterpret_cast<float*>(sm + P::STAGES * P::STAGE);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + P::STAGES * P::STAGE + PAIR_EPI_WARPS * TURN_BYTES);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * PAIR_MAX_STAGES + 5);
+  volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = (int)cluster_rank(), pair = (int)blockIdx.x >> 1, npairs = (int)gridDim.x >> 1;
+  const uint32_t full = smem_u32(bars), stage_free = full + 8 * PAIR_MAX_STAGES, acc_full = stage_free + 8 * PAIR_MAX_STAGES,
+                 acc_free = acc_full + 16, drained = acc_free + 16;
+  const int items = a.m_tiles * a.n_tiles;
+
+  if (tid == 0) {
+    *dead = 0;
+    for (int i = 0; i < P::STAGES; ++i) { mbar_init(full + 8 * i, 1); mbar_init(stage_free + 8 * i, 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_free + 8 * i, 2 * PAIR_EPI_WARPS); }
+    mbar_init(drained, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) pair_tmem_alloc(smem_u32(tmem_slot), P::TMEM);
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+
+  // Tiles in groups of m_group activation tiles, activation tiles fastest within a group: the pairs that run together share their
+  // weight rows in L2, and a group's activation rows stay there while the weights go by.
+  auto split = [&](int item, int& mt, int& nt) {
+    const int g = item / (a.m_group * a.n_tiles), first = g * a.m_group, height = min(a.m_group, a.m_tiles - first);
+    const int at = item - first * a.n_tiles;
+    nt = at / height;
+    mt = first + at - nt * height;
+  };
+
+  if (warp < PAIR_EPI_WARPS) {
+    // ---- epilogue: warp w reads TMEM lanes 32 (w % 4) .. of this CTA's 128 activation rows, one half of the weight rows
+    constexpr int HALF = NW / 2;
+    const int quad = warp & 3, side = warp >> 2;
+    float* mine = turn + warp * (TURN_BYTES / 4);
+    int k = 0;  // blocks of K so far, over all tiles
+    bool alive = true;
+    pdl_wait();
+    for (int item = pair; item < items && alive; item += npairs) {
+      int mt, nt;
+      split(item, mt, nt);
+      const int m_first = mt * 256 + rank * 128 + quad * 32, n_first = nt * NW + side * HALF;
+      const float* sx = a.sx + (size_t)min(m_first + lane, a.out.m - 1) * a.kblocks;
+      const float* sw = a.sw + (size_t)min(n_first / F8_BLOCK, (a.out.n - 1) / F8_BLOCK) * a.kblocks;
+      float2 acc[HALF / 2];
+#pragma unroll
+      for (int i = 0; i < HALF / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+      float s = sx[0] * sw[0];
+#pragma unroll 1
+      for (int kb = 0; kb < a.kblocks; ++kb, ++k) {
+        const int buf = k & 1;
+        const float now = s;
+        if (kb + 1 < a.kblocks) s = sx[kb + 1] * sw[kb + 1];  // in flight beside the wait
+        if (!(alive = w_wait(acc_full + 8 * buf, (uint32_t)((k >> 1) & 1), dead, a.status))) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t tl = tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(buf * NW + side * HALF);
+        uint32_t v[2][16];
+        x_ld16(tl, v[0]);
+#pragma unroll
+        for (int c = 0; c < HALF / 16; ++c) {
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          if (c + 1 < HALF / 16) x_ld16(tl + 16 * (c + 1), v[(c + 1) & 1]);
+          else {
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) cluster_arrive(acc_free + 8 * buf, 0);
+          }
+          const float2 ss = make_float2(now, now);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            acc[8 * c + i] = fma2(make_float2(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])), ss, acc[8 * c + i]);
+        }
+      }
+      if (!alive) break;
+      // out, 16 columns at a time, turned in shared memory so that a row's columns leave together
+#pragma unroll
+      for (int c = 0; c < HALF / 16; ++c) {
+        if (n_first + 16 * c >= a.out.n) break;
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<float4*>(mine + lane * TURN_ROW + 4 * i) =
+              make_float4(acc[8 * c + 2 * i].x, acc[8 * c + 2 * i].y, acc[8 * c + 2 * i + 1].x, acc[8 * c + 2 * i + 1].y);
+        __syncwarp();
+        const int n = n_first + 16 * c + 4 * (lane & 3);
+#pragma unroll 1
+        for (int r = lane >> 2; r < 32 && m_first + r < a.out.m; r += 8) {
+          const float4 v = *reinterpret_cast<const float4*>(mine + r * TURN_ROW + 4 * (lane & 3));
+          if (a.vec) {  // whole fours: n is a multiple of four then
+            if (n < a.out.n) f8_put4(a.out, v, m_first + r, n);
+          } else {
+            const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (n + i < a.out.n) f8_put(a.out, e[i], m_first + r, n + i);
+          }
+        }
+      }
+    }
+  } else if (warp == PAIR_EPI_WARPS) {
+    // ---- copy requester: a stage is one block of K, 128 activation rows and NW / 2 weight rows per CTA; the copies of both CTAs are
+    // counted on the even CTA's barrier
+    if (lane == 0) {
+      pdl_wait();
+      int k = 0;
+      bool alive = true;
+      for (int item = pair; item < items && alive; item += npairs) {
+        int mt, nt;
+        split(item, mt, nt);
+        const int xr = mt * 256 + rank * 128, wr = nt * NW + rank * (NW / 2);
+        for (int kb = 0; kb < a.kblocks; ++kb, ++k) {
+          const int s = k % P::STAGES, round = k / P::STAGES;
+          if (round > 0 && !(alive = x_wait(stage_free + 8 * s, (uint32_t)((round - 1) & 1), dead, a.status))) break;
+          const uint32_t dst = smem_u32(sm + s * P::STAGE), bar = cluster_addr(full + 8 * s, 0);
+          if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * P::STAGE);
+          pair_tma_box2(dst, &xmap, kb * F8_BLOCK, xr, bar);
+          pair_tma_box2(dst + F8_A_BYTES, &wmap, kb * F8_BLOCK, wr, bar);
+        }
+      }
+      if (*dead) {
+        // the even CTA waits for the copies that its barriers count; the odd one has no barrier of its own that counts
+        // them and lets the limit of a wait run out instead, which takes far longer than a copy
+        if (rank) x_drain(full, 0);
+        else
+          for (int i = max(0, k - P::STAGES); i < k; ++i) x_drain(full + 8 * (i % P::STAGES), (uint32_t)((i / P::STAGES) & 1));
+      }
+    }
+  } else {
+    // ---- MMA issuer (even CTA): a block of K per accumulator; the next stage's barrier is polled before this one's MMAs are issued
+    int s = 0, k = 0;
+    uint32_t parity = 0, ready = 0;
+    bool alive = rank == 0;
+    const uint64_t adesc0 = x_desc_rows(smem_u32(sm)), bdesc0 = x_desc_rows(smem_u32(sm) + F8_A_BYTES);
+    for (int item = pair; item < items && alive; item += npairs) {
+      for (int kb = 0; kb < a.kblocks && alive; ++kb, ++k) {
+        const int buf = k & 1;
+        if (!__all_sync(0xFFFFFFFFu, ready) && !(alive = w_wait(full + 8 * s, parity, dead, a.status))) break;
+        if (k >= 2 && !(alive = w_wait(acc_free + 8 * buf, (uint32_t)(((k >> 1) - 1) & 1), dead, a.status))) break;
+        const int now = s;
+        if (++s == P::STAGES) { s = 0; parity ^= 1u; }
+        ready = x_poll(full + 8 * s, parity);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t at = (uint64_t)((now * P::STAGE) >> 4);
+        pair_mma4_f8<2>(tmem + (uint32_t)(buf * NW), adesc0 + at, bdesc0 + at, P::IDESC, 0u);
+        pair_commit(stage_free + 8 * now);
+        pair_commit(acc_full + 8 * buf);
+      }
+    }
+    if (rank == 0) pair_commit(drained);
+    x_drain(drained, 0);
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  cluster_sync();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (warp == 0) pair_tmem_free(tmem, P::TMEM);
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------
+
+struct F8Job {
+  const uint8_t* x;
+  size_t ld;
+  const float* sx;
+  const fb200_f8matrix* w;
+  F8Out out;
+  int kblocks;
+};
+
+template <typename K>
+int allow_smem(fb200_device* dev, K kern, int bytes, bool (&configured)[64]) {
+  if (configured[dev->ordinal & 63]) return FB200_OK;
+  FB_CUDA(dev, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  configured[dev->ordinal & 63] = true;
+  return FB200_OK;
+}
+
+template <int BM>
+int launch_few(fb200_device* dev, const F8Job& j, int split) {
+  using F = Few<BM>;
+  static bool configured[64] = {false};
+  int rc = allow_smem(dev, f8_few_kernel<BM>, F::SMEM, configured);
+  if (rc) return rc;
+  CUtensorMap xmap;
+  if (!fb200_make_map_2d_bytes(&xmap, j.x, j.w->k, (uint64_t)j.out.m, j.ld, BM))
+    return fb200_fail(dev, FB200_ERR_CUDA, "f8_mat_mul: tensor map refused (x %d rows every %zu bytes)", j.out.m, j.ld);
+  const FewArgs a = {j.sx, j.w->scales, j.out, j.kblocks, (j.out.m + BM - 1) / BM, split, dev->status};
+  const long long ctas = (long long)a.m_tiles * ((j.out.n + 127) / 128) * split;
+  if (ctas > 0x7FFFFFFF) return fb200_fail(dev, FB200_ERR_INVALID_SHAPE, "f8_mat_mul: %d x %d outputs are too many", j.out.m, j.out.n);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(F::THREADS);
+  cfg.dynamicSmemBytes = F::SMEM;
+  cfg.stream = dev->stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dev->pdl ? 2 : 1;
+  FB_CUDA(dev, cudaLaunchKernelEx(&cfg, f8_few_kernel<BM>, a, j.w->map128, xmap));
+  dev->launches++;
+  return FB200_OK;
+}
+
+template <int NW>
+int launch_pair(fb200_device* dev, const F8Job& j) {
+  using P = Pair<NW>;
+  static bool configured[64] = {false};
+  int rc = allow_smem(dev, f8_pair_kernel<NW>, P::SMEM, configured);
+  if (rc) return rc;
+  CUtensorMap xmap;
+  if (!fb200_make_map_2d_bytes(&xmap, j.x, j.w->k, (uint64_t)j.out.m, j.ld, 128))
+    return fb200_fail(dev, FB200_ERR_CUDA, "f8_mat_mul: tensor map refused (x %d rows every %zu bytes)", j.out.m, j.ld);
+  PairArgs a = {j.sx, j.w->scales, j.out, j.kblocks, (j.out.m + 255) / 256, (j.out.n + NW - 1) / NW, 1, 0, dev->status};
+  const long long items = (long long)a.m_tiles * a.n_tiles;
+  if (items > 0x3FFFFFFF) return fb200_fail(dev, FB200_ERR_INVALID_SHAPE, "f8_mat_mul: %d x %d outputs are too many", j.out.m, j.out.n);
+  // the activation rows of a group take at most 32 MB of L2
+  const long long fit = (32ll << 20) / (256ll * F8_BLOCK * j.kblocks);
+  a.m_group = fit < 1 ? 1 : fit > a.m_tiles ? a.m_tiles : (int)fit;
+  const uintptr_t four = j.out.type == FB200_F32 ? 16 : 8;
+  a.vec = j.out.n % 4 == 0 && (uintptr_t)j.out.y % four == 0 && (uintptr_t)j.out.r1 % 16 == 0 && (uintptr_t)j.out.r2 % 16 == 0;
+  const int pairs = items < dev->sm_count / 2 ? (int)items : dev->sm_count / 2;
+  return fb200_launch(dev, f8_pair_kernel<NW>, dim3((unsigned)(2 * pairs)), dim3(PAIR_THREADS), (size_t)P::SMEM, true, a,
+                      NW == 256 ? j.w->map128 : j.w->map64, xmap);
+}
+
+int f8_product(fb200_device* dev, const F8Job& j) {
+  const int m = j.out.m, n_tiles = (j.out.n + 127) / 128;
+  int bm = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128, split = 1;
+  const int tiles = n_tiles * ((m + bm - 1) / bm);
+  while (split < 8 && tiles * split * 2 <= dev->sm_count * (bm <= 64 ? 2 : 1) && j.kblocks >= split * 4) split *= 2;
+  if (m > 256) bm = 256, split = 2;
+  // FB200_F8_TILE="BM,SPLIT": activation rows and ranges of K of the kernel for few rows; "256,1" / "256,2": pairs with 128 / 256 weight
+  // rows (tests, tuning; read per call)
+  int fbm, fsplit;
+  if (const char* cfg = getenv("FB200_F8_TILE"))
+    if (sscanf(cfg, "%d,%d", &fbm, &fsplit) == 2) bm = fbm, split = fsplit;
+  if (split != 1 && split != 2 && split != 4 && split != 8) split = 1;
+  switch (bm) {
+    case 16: return launch_few<16>(dev, j, split);
+    case 32: return launch_few<32>(dev, j, split);
+    case 64: return launch_few<64>(dev, j, split);
+    case 128: return launch_few<128>(dev, j, split);
+    default: return split == 1 ? launch_pair<128>(dev, j) : launch_pair<256>(dev, j);
+  }
+}
+
+int check_shape(fb200_device* dev, const char* op, const uint64_t* shape, int rank) {
+  if (rank != 2 || !shape) return fb200_fail(dev, FB200_ERR_INVALID_SHAPE, "%s: needs a rank-2 shape, got rank %d", op, rank);
+  if (!shape[0] || !shape[1] || shape[0] > (1ull << 27) || shape[1] > (1ull << 27))
+    return fb200_fail(dev, FB200_ERR_INVALID_SHAPE, "%s: shape [%llu, %llu]", op, (unsigned long long)shape[0], (unsigned long long)shape[1]);
+  return FB200_OK;
+}
+
+int make_maps(fb200_device* dev, fb200_f8matrix* w) {
+  if (fb200_make_map_2d_bytes(&w->map128, w->codes, w->k, w->n, w->ld, 128) && fb200_make_map_2d_bytes(&w->map64, w->codes, w->k, w->n, w->ld, 64))
+    return FB200_OK;
+  return fb200_fail(dev, FB200_ERR_CUDA, "F8Matrix: tensor map refused (%llu x %llu)", (unsigned long long)w->n, (unsigned long long)w->k);
+}
+
+}  // namespace
+
+extern "C" {
+
+int fb200_f8matrix_from_raw_bytes(fb200_device* dev, const uint64_t* shape, int rank, const void* codes_host, size_t nbytes, const float* scales_host,
+                                  size_t nscales, fb200_f8matrix** out) {
+  int rc = fb200_bind(dev);
+  if (rc) return rc;
+  if (!out) return fb200_fail(dev, FB200_ERR_INVALID_ARGUMENT, "out is null");
+  *out = nullptr;
+  if ((rc = check_shape(dev, "F8Matrix", shape, rank))) return rc;
+  const uint64_t n = shape[0], k = shape[1], blocks = ((n + 127) / 128) * ((k + 127) / 128);
+  if (!codes_host || !scales_host) return fb200_fail(dev, FB200_ERR_INVALID_ARGUMENT, "F8Matrix: null argument");
+  if (nbytes != n * k || nscales != blocks)
+    return fb200_fail(dev, FB200_ERR_INVALID_SHAPE, "F8Matrix: shape [%llu, %llu] needs %llu codes and %llu scales, got %zu and %zu", (unsigned long long)n,
+                      (unsigned long long)k, (unsigned long long)(n * k), (unsigned long long)blocks, nbytes, nscales);
+  fb200_f8matrix* w = new (std::nothrow) fb200_f8matrix();
+  if (!w) return fb200_fail(dev, FB200_ERR_CAPACITY, "F8Matrix: no host memory");
+  w->dev = dev; w->n = n; w->k = k; w->ld = (k + 15) / 16 * 16; w->owned = true;
+  cudaError_t e = cudaMalloc(&w->codes, n * w->ld);
+  if (e == cudaSuccess) e = cudaMalloc(&w->scales, blocks * sizeof(float));
+  if (e == cudaSuccess) e = cudaMemcpy2DAsync(w->codes, w->ld, codes_host, k, k, n, cudaMemcpyHostToDevice, dev->stream);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(w->scales, scales_host, blocks * sizeof(float), cudaMemcpyHostToDevice, dev->stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(dev->stream);
+  rc = e == cudaSuccess ? make_maps(dev, w) : fb200_fail(dev, FB200_ERR_CUDA, "F8Matrix upload: %s", cudaGetErrorString(e));
+  if (e != cudaSuccess) cudaGetLastError();  // reported here, not by the check of a later launch
+  if (rc) {
+    cudaFree(w->codes);
+    cudaFree(w->scales);
+    delete w;
+    return rc;
+  }
+  *out = w;
+  return FB200_OK;
+}
+
+int fb200_f8matrix_from_device(fb200_device* dev, const uint64_t* shape, int rank, const uint8_t* codes_dev, size_t ld, const float* scales_dev,
+                               fb200_f8matrix** out) {
+  int rc = fb200_bind(dev);
+  if (rc) return rc;
+  if (!out) return fb200_fail(dev, FB200_ERR_INVALID_ARGUMENT, "out is null");
+  *out = nullptr;
+  if ((rc = check_shape(dev, "F8Matrix", shape, rank))) return rc;
+  if (!codes_dev || !scales_dev) return fb200_fail(dev, FB200_ERR_INVALID_ARGUMENT, "F8Matrix: null argument");
+  if (ld < shape[1] || ld % 16 || (uintptr_t)codes_dev % 16 || (uintptr_t)scales_dev % 4)
+    return fb200_fail(dev, FB200_ERR_INVALID_SHAPE, "F8Matrix: rows of %llu codes every %zu bytes (a multiple of 16, from a multiple of 16 on)",
+                      (unsigned long long)shape[1], ld);
+  fb200_f8matrix* w = new (std::nothrow) fb200_f8matrix();
+  if (!w) return fb200_fail(dev, FB200_ERR_CAPACITY, "F8Matrix: no host memory");
+  w->dev = dev; w->n = shape[0]; w->k = shape[1]; w->ld = ld;
+  w->codes = const_cast<uint8_t*>(codes_dev); w->scales = const_cast<float*>(scales_dev);
+  // products fetch the codes without waiting for the kernel in front of them: what writes them has to be done
+  const cudaError_t e = cudaStreamSynchronize(dev->stream);
+  rc = e == cudaSuccess ? make_maps(dev, w) : fb200_fail(dev, FB200_ERR_CUDA, "F8Matrix: %s", cudaGetErrorString(e));
+  if (rc) {
+    delete w;
+    return rc;
+  }
+  *out = w;
+  return FB200_OK;
+}
+
+int fb200_f8matrix_free(fb200_f8matrix* w) {
+  if (!w) return FB200_OK;
+  const int rc = fb200_bind(w->dev);
+  if (rc) return rc;
+  if (w->owned) {
+    cudaStreamSynchronize(w->dev->stream);
+    cudaFree(w->codes);
+    cudaFree(w->scales);
+  }
+  delete w;
+  return FB200_OK;
+}
+
+int fb200_f8matrix_shape(const fb200_f8matrix* w, uint64_t* n_out, uint64_t* k_out) {
+  if (!w) return FB200_ERR_INVALID_ARGUMENT;
+  if (n_out) *n_out = w->n;
+  if (k_out) *k_out = w->k;
+  return FB200_OK;
+}
+
+int fb200_f8_mat_mul(fb200_device* dev, const uint8_t* codes_dev, size_t ld, const float* scales_dev, size_t m, const fb200_f8matrix* w, uint32_t y_type,
+                     void* y_dev, const fb200_epilogue* ep) {
+  const int rc = fb200_bind(dev);
+  if (rc) return rc;
+  if (!w || !codes_dev || !scales_dev || !y_dev) return fb200_fail(dev, FB200_ERR_INVALID_ARGUMENT, "f8_mat_mul: null argument");
+  if (w->dev != dev) return fb200_fail(dev, FB200_ERR_DEVICE_MISMATCH, "f8_mat_mul: weight lives on another device handle");
+  if (y_type != FB200_F32 && y_type != FB200_F16 && y_type != FB200_BF16)
+    return fb200_fail(dev, FB200_ERR_UNSUPPORTED_DTYPE, "f8_mat_mul: outputs of type %u (F32, F16 or BF16)", y_type);
+  const int epi = ep ? ep->kind : FB200_EPI_NONE;
+  if (epi < 0 || epi > 3) return fb200_fail(dev, FB200_ERR_INVALID_ARGUMENT, "f8_mat_mul: epilogue kind %d", epi);
+  if (epi == FB200_EPI_SWIGLU)
+    return fb200_fail(dev, FB200_ERR_UNSUPPORTED_DTYPE, "f8_mat_mul: no SwiGLU epilogue (fb200_silu_mul_f8 takes the product's rows)");
+  if (epi != FB200_EPI_NONE && !ep->r1_dev) return fb200_fail(dev, FB200_ERR_INVALID_ARGUMENT, "f8_mat_mul: residual / bias epilogue without r1");
+  if (epi == FB200_EPI_BIAS && ep->r2_dev) return fb200_fail(dev, FB200_ERR_INVALID_ARGUMENT, "f8_mat_mul: the bias epilogue takes r1 only");
+  if (m > (1ull << 27)) return fb200_fail(dev, FB200_ERR_INVALID_SHAPE, "f8_mat_mul: %zu rows are too many", m);
+  if (ld < w->k || ld % 16 || (uintptr_t)codes_dev % 16 || (uintptr_t)scales_dev % 4 || (uintptr_t)y_dev % (y_type == FB200_F32 ? 4 : 2))
+    return fb200_fail(dev, FB200_ERR_INVALID_SHAPE, "f8_mat_mul: rows of %llu codes every %zu bytes (a multiple of 16, from a multiple of 16 on)",
+                      (unsigned long long)w->k, ld);
+  if (epi != FB200_EPI_NONE && ((uintptr_t)ep->r1_dev % 4 || (uintptr_t)ep->r2_dev % 4))
+    return fb200_fail(dev, FB200_ERR_INVALID_ARGUMENT, "f8_mat_mul: r1 or r2 is not aligned");
+  if (m == 0) return FB200_OK;
+  F8Job j = {codes_dev, ld, scales_dev, w, {y_dev, y_type, nullptr, nullptr, nullptr, (int)m, (int)w->n}, (int)((w->k + 127) / 128)};
+  if (epi == FB200_EPI_BIAS) j.out.bias = ep->r1_dev;
+  if (epi == FB200_EPI_RESIDUAL) { j.out.r1 = ep->r1_dev; j.out.r2 = ep->r2_dev; }
+  fb200_op_trace scope(dev, m <= 32 ? "f8_mat_mul (1..32 rows)" : "f8_mat_mul (> 32 rows)",
+                       (double)w->n * (double)w->k + (double)m * ((double)w->k + (y_type == FB200_F32 ? 4.0 : 2.0) * (double)w->n));
+  return f8_product(dev, j);
+}
+
+}  // extern "C"
