@@ -65,8 +65,9 @@ struct Few {
   static constexpr int EPI_WARPS = BM >= 64 ? 8 : 4, THREADS = (EPI_WARPS + 2) * 32;
   static constexpr int COLS = BM * 4 / EPI_WARPS;  // activation rows of an epilogue thread
   static constexpr int STAGE = F8_A_BYTES + BM * 128;
-  static constexpr int STAGES = BM == 16 ? 6 : BM == 32 ? 5 : BM == 64 ? 4 : 6;
-  static constexpr int BUFS = 4, TMEM = BUFS * BM;
+  // every stage of operands has an accumulator of its own, so that one arrival tells both rings that a block is multiplied
+  static constexpr int STAGES = BM == 16 ? 6 : BM == 32 ? 5 : 4;
+  static constexpr int TMEM = BM == 16 ? 128 : BM == 32 ? 256 : STAGES * BM;
   static constexpr int SCALE_ROW = BM + 4, SCALE_BYTES = 2 * FEW_SCALES * SCALE_ROW * 4;
   static constexpr int SMEM = STAGES * STAGE + SCALE_BYTES + 256 + 1024;
   static constexpr int PER_SM = BM <= 64 ? 2 : 1;
@@ -97,10 +98,9 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~(uintptr_t)1023);
   float* scales = reinterpret_cast<float*>(sm + F::STAGES * F::STAGE);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + F::STAGES * F::STAGE + F::SCALE_BYTES);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * F::STAGES + 2 * F::BUFS + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * F::STAGES + 1);
   volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const uint32_t full = smem_u32(bars), stage_free = full + 8 * F::STAGES, acc_full = stage_free + 8 * F::STAGES, acc_free = acc_full + 8 * F::BUFS,
-                 drained = acc_free + 8 * F::BUFS;
+  const uint32_t full = smem_u32(bars), multiplied = full + 8 * F::STAGES, acc_free = multiplied + 8 * F::STAGES, drained = acc_free + 8 * F::STAGES;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = (int)cluster_rank(), tile = (int)blockIdx.x / a.split;
   // activation tiles fastest: the CTAs that run together share their weight rows in L2
@@ -109,8 +109,7 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
 
   if (tid == 0) {
     *dead = 0;
-    for (int i = 0; i < F::STAGES; ++i) { mbar_init(full + 8 * i, 1); mbar_init(stage_free + 8 * i, 1); }
-    for (int i = 0; i < F::BUFS; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_free + 8 * i, F::EPI_WARPS); }
+    for (int i = 0; i < F::STAGES; ++i) { mbar_init(full + 8 * i, 1); mbar_init(multiplied + 8 * i, 1); mbar_init(acc_free + 8 * i, F::EPI_WARPS); }
     mbar_init(drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -146,8 +145,10 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
     };
     pdl_wait();
     fetch(0);
+    int st = 0;
+    uint32_t parity = 0;
     for (int i = 0; i < nkb; ++i) {
-      const int buf = i % F::BUFS, at = i % FEW_SCALES;
+      const int at = i % FEW_SCALES;
       if (at == 0) {
         // the other half was last read before everybody came to this barrier's predecessor
         float* half = scales + ((i / FEW_SCALES) & 1) * FEW_SCALES * F::SCALE_ROW;
@@ -156,27 +157,28 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
         asm volatile("bar.sync 1, %0;" ::"n"(ET) : "memory");
         if (i + FEW_SCALES < nkb) fetch(i + FEW_SCALES);
       }
-      if (!w_wait(acc_full + 8 * buf, (uint32_t)((i / F::BUFS) & 1), dead, a.status)) {
+      if (!f_wait(multiplied + 8 * st, parity, dead, a.status)) {
         // the barriers of the scales to come are met all the same
         for (int j = (i / FEW_SCALES + 1) * FEW_SCALES; j < nkb; j += FEW_SCALES) asm volatile("bar.sync 1, %0;" ::"n"(ET) : "memory");
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t tl = tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(buf * BM + col0);
+      const uint32_t tl = tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(st * BM + col0), freed = acc_free + 8 * st;
       uint32_t v[F::COLS / 16][16];
 #pragma unroll
       for (int j = 0; j < F::COLS / 16; ++j) x_ld16(tl + 16 * j, v[j]);
+      if (++st == F::STAGES) { st = 0; parity ^= 1u; }
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(acc_free + 8 * buf);
+      w_arrive(freed);
       const float4* sc = reinterpret_cast<const float4*>(scales + (((i / FEW_SCALES) & 1) * FEW_SCALES + at) * F::SCALE_ROW + col0);
 #pragma unroll
       for (int j = 0; j < F::COLS / 4; ++j) {
-        const float4 s = sc[j];
+        const float4 f = sc[j];
         const uint32_t* p = &v[j / 4][4 * (j % 4)];
-        acc[2 * j] = fma2(make_float2(__uint_as_float(p[0]), __uint_as_float(p[1])), make_float2(s.x, s.y), acc[2 * j]);
-        acc[2 * j + 1] = fma2(make_float2(__uint_as_float(p[2]), __uint_as_float(p[3])), make_float2(s.z, s.w), acc[2 * j + 1]);
+        acc[2 * j] = fma2(make_float2(__uint_as_float(p[0]), __uint_as_float(p[1])), make_float2(f.x, f.y), acc[2 * j]);
+        acc[2 * j + 1] = fma2(make_float2(__uint_as_float(p[2]), __uint_as_float(p[3])), make_float2(f.z, f.w), acc[2 * j + 1]);
       }
     }
   } else if (warp == F::EPI_WARPS) {
@@ -192,7 +194,7 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
       for (; i < pre; ++i) x_tma_box2(smem_u32(sm + i * F::STAGE + F8_A_BYTES), &xmap, (kb0 + i) * F8_BLOCK, m0, full + 8 * i);
       for (; i < nkb; ++i) {
         const int s = i % F::STAGES;
-        if (!x_wait(stage_free + 8 * s, (uint32_t)((i / F::STAGES - 1) & 1), dead, a.status)) break;
+        if (!x_wait(multiplied + 8 * s, (uint32_t)((i / F::STAGES - 1) & 1), dead, a.status)) break;
         const uint32_t dst = smem_u32(sm + s * F::STAGE), bar = full + 8 * s;
         mbar_expect_tx(bar, F::STAGE);
         x_tma_box2(dst, &wmap, (kb0 + i) * F8_BLOCK, nt * 128, bar);
@@ -202,18 +204,21 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
         for (int j = max(0, i - F::STAGES); j < i; ++j) x_drain(full + 8 * (j % F::STAGES), (uint32_t)((j / F::STAGES) & 1));
     }
   } else {
-    // ---- MMA issuer
+    // ---- MMA issuer; the next block's barriers are polled before this one's MMAs are issued
     const uint64_t adesc0 = x_desc_rows(smem_u32(sm)), bdesc0 = x_desc_rows(smem_u32(sm) + F8_A_BYTES);
-    bool alive = true;
-    for (int i = 0; i < nkb && alive; ++i) {
-      const int s = i % F::STAGES, buf = i % F::BUFS;
-      if (i >= F::BUFS && !(alive = w_wait(acc_free + 8 * buf, (uint32_t)((i / F::BUFS - 1) & 1), dead, a.status))) break;
-      if (!(alive = w_wait(full + 8 * s, (uint32_t)((i / F::STAGES) & 1), dead, a.status))) break;
+    int st = 0;
+    uint32_t parity = 0, ready = 0, room = 1;  // a buffer's first use waits for nobody
+    for (int i = 0; i < nkb; ++i) {
+      if (!__all_sync(0xFFFFFFFFu, room) && !f_wait(acc_free + 8 * st, parity ^ 1u, dead, a.status)) break;
+      if (!__all_sync(0xFFFFFFFFu, ready) && !f_wait(full + 8 * st, parity, dead, a.status)) break;
+      const int now = st;
+      if (++st == F::STAGES) { st = 0; parity ^= 1u; }
+      ready = x_poll(full + 8 * st, parity);
+      room = i + 1 < F::STAGES ? 1u : x_poll(acc_free + 8 * st, parity ^ 1u);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint64_t at = (uint64_t)((s * F::STAGE) >> 4);
-      w_mma4_f8<2, 2>(tmem + (uint32_t)(buf * BM), adesc0 + at, bdesc0 + at, F::IDESC, 0u);
-      w_commit(stage_free + 8 * s);
-      w_commit(acc_full + 8 * buf);
+      const uint64_t at = (uint64_t)((now * F::STAGE) >> 4);
+      w_mma4_f8<2, 2>(tmem + (uint32_t)(now * BM), adesc0 + at, bdesc0 + at, F::IDESC, 0u);
+      w_commit(multiplied + 8 * now);
     }
     w_commit(drained);
     x_drain(drained, 0);
@@ -252,25 +257,34 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
 
 // ---- many activation rows -----------------------------------------------------------------------------------------------
 
-constexpr int PAIR_EPI_WARPS = 8, PAIR_THREADS = (PAIR_EPI_WARPS + 2) * 32, PAIR_MAX_STAGES = 8;
-constexpr int TURN_ROW = 20, TURN_BYTES = 32 * TURN_ROW * 4;  // a warp's 32 rows x 16 columns on their way out, rows 80 bytes apart
+// Two warpgroups of epilogue warps and one of the copy requester and the issuer, which hands its registers over: 384 x 168 at launch are
+// 256 x 224 + 128 x 56. A thread holds 128 sums and 64 values on their way.
+constexpr int PAIR_EPI_WARPS = 8, PAIR_THREADS = (PAIR_EPI_WARPS + 4) * 32, PAIR_MAX_STAGES = 8;
+constexpr int TURN_BYTES = 32 * 128;  // a warp's 32 rows x 128 bytes on their way out, 16-byte piece p of row r at place p ^ (r % 8)
 
 template <int NW>
 struct Pair {
-  static constexpr int STAGE = F8_A_BYTES + NW / 2 * 128, STAGES = NW == 256 ? 6 : 8, TMEM = 2 * NW;
+  static constexpr int STAGE = F8_A_BYTES + NW / 2 * 128, STAGES = NW == 256 ? 6 : 8, TMEM = 512;
+  static constexpr int PARTS = NW / 128, BUFS = 4 / PARTS;  // four accumulators of 128 columns: PARTS of a block of K, BUFS blocks
   static constexpr int SMEM = STAGES * STAGE + PAIR_EPI_WARPS * TURN_BYTES + 256 + 1024;
-  // instruction descriptor: f32 accumulator, e4m3 A and B, both K-major, N = NW, M = 256 over the pair
-  static constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(NW >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+  // instruction descriptor: f32 accumulator, e4m3 A and B, both K-major, N = 128, M = 256 over the pair
+  static constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
 };
 
 struct PairArgs {
   const float *sx, *sw;
   F8Out out;
   int kblocks, m_tiles, n_tiles, m_group;
-  int vec;  // four columns of y (and of the residuals) are aligned
+  int vec;   // four columns of y (and of the residuals) are aligned
+  int pack;  // 16-bit y without residual or bias, eight columns aligned: rounded before they are turned
   int* status;
 };
 
+__device__ __forceinline__ uint32_t f8_pair(const F8Out& o, float2 v) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(v.x, v.y);
+  const __half2 h = __floats2half2_rn(v.x, v.y);
+  return o.type == FB200_BF16 ? *reinterpret_cast<const uint32_t*>(&b) : *reinterpret_cast<const uint32_t*>(&h);
+}
 // Four neighbouring outputs
 __device__ __forceinline__ void f8_put4(const F8Out& o, float4 v, int m, int n) {
   const size_t at = (size_t)m * o.n + n;
@@ -279,12 +293,59 @@ __device__ __forceinline__ void f8_put4(const F8Out& o, float4 v, int m, int n) 
   if (o.r2) { const float4 r = *reinterpret_cast<const float4*>(o.r2 + at); v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w; }
   if (o.type == FB200_F32) {
     *reinterpret_cast<float4*>(reinterpret_cast<float*>(o.y) + at) = v;
-  } else if (o.type == FB200_BF16) {
-    const __nv_bfloat162 p = __floats2bfloat162_rn(v.x, v.y), q = __floats2bfloat162_rn(v.z, v.w);
-    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(o.y) + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&p), *reinterpret_cast<const uint32_t*>(&q));
   } else {
-    const __half2 p = __floats2half2_rn(v.x, v.y), q = __floats2half2_rn(v.z, v.w);
-    *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(o.y) + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&p), *reinterpret_cast<const uint32_t*>(&q));
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(o.y) + at) = make_uint2(f8_pair(o, make_float2(v.x, v.y)), f8_pair(o, make_float2(v.z, v.w)));
+  }
+}
+
+// A warp's 32 rows from m0 on, COLS columns from n0 on, a row per thread, to y: turned in shared memory, so that a row's columns leave
+// together.
+template <int COLS>
+__device__ __forceinline__ void f8_store_rows(const PairArgs& a, const float2 (&acc)[COLS / 2], uint8_t* turn, int m0, int n0) {
+  const int lane = threadIdx.x & 31, m_end = a.out.m - m0, n_end = a.out.n - n0;
+  if (a.pack) {
+    const uint8_t* from = turn + (lane >> 3) * 128;
+    uint16_t* to = reinterpret_cast<uint16_t*>(a.out.y) + (size_t)m0 * a.out.n + n0 + 8 * (lane & 7);
+#pragma unroll
+    for (int c = 0; c < COLS / 64; ++c) {
+      if (64 * c >= n_end) break;
+      __syncwarp();
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        const float2* v = acc + 32 * c + 4 * p;
+        *reinterpret_cast<uint4*>(turn + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_uint4(f8_pair(a.out, v[0]), f8_pair(a.out, v[1]), f8_pair(a.out, v[2]), f8_pair(a.out, v[3]));
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3);
+        const uint4 v = *reinterpret_cast<const uint4*>(from + 512 * i + (((lane & 7) ^ (r & 7)) << 4));
+        if (r < m_end && 64 * c + 8 * (lane & 7) < n_end) *reinterpret_cast<uint4*>(to + (size_t)r * a.out.n + 64 * c) = v;
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int c = 0; c < COLS / 32; ++c) {
+    if (32 * c >= n_end) break;
+    __syncwarp();
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      const float2* v = acc + 16 * c + 2 * p;
+      *reinterpret_cast<float4*>(turn + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+    }
+    __syncwarp();
+    if (a.vec) {  // whole fours: N is a multiple of four then
+#pragma unroll 2
+      for (int r = lane >> 3; r < 32 && r < m_end; r += 4)
+        if (32 * c + 4 * (lane & 7) < n_end)
+          f8_put4(a.out, *reinterpret_cast<const float4*>(turn + r * 128 + (((lane & 7) ^ (r & 7)) << 4)), m0 + r, n0 + 32 * c + 4 * (lane & 7));
+    } else {
+#pragma unroll 2
+      for (int r = 0; r < 32 && r < m_end; ++r)
+        if (32 * c + lane < n_end)
+          f8_put(a.out, *reinterpret_cast<const float*>(turn + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3)), m0 + r, n0 + 32 * c + lane);
+    }
   }
 }
 
@@ -295,21 +356,21 @@ f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const
   extern __shared__ uint8_t sm_raw[];
   // the same offset in both CTAs: their dynamic shared memory starts at the same address
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~(uintptr_t)1023);
-  float* turn = reinterpret_cast<float*>(sm + P::STAGES * P::STAGE);
+  uint8_t* turn = sm + P::STAGES * P::STAGE;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + P::STAGES * P::STAGE + PAIR_EPI_WARPS * TURN_BYTES);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * PAIR_MAX_STAGES + 5);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * PAIR_MAX_STAGES + 9);
   volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = (int)cluster_rank(), pair = (int)blockIdx.x >> 1, npairs = (int)gridDim.x >> 1;
   const uint32_t full = smem_u32(bars), stage_free = full + 8 * PAIR_MAX_STAGES, acc_full = stage_free + 8 * PAIR_MAX_STAGES,
-                 acc_free = acc_full + 16, drained = acc_free + 16;
+                 acc_free = acc_full + 32, drained = acc_free + 32;
   const int items = a.m_tiles * a.n_tiles;
 
   if (tid == 0) {
     *dead = 0;
-    for (int i = 0; i < P::STAGES; ++i) { mbar_init(full + 8 * i, 1); mbar_init(stage_free + 8 * i, 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_free + 8 * i, 2 * PAIR_EPI_WARPS); }
-    mbar_init(drained, 1);
+    for (int i = 0; i < P::STAGES; ++i) { mbar_init(full + 8 * i, 1); mbar_init(stage_free + 8 * i, P::PARTS); }
+    for (int i = 0; i < 4; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_free + 8 * i, 2 * PAIR_EPI_WARPS / P::PARTS); }
+    mbar_init(drained, 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) pair_tmem_alloc(smem_u32(tmem_slot), P::TMEM);
@@ -330,74 +391,69 @@ f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const
 
   if (warp < PAIR_EPI_WARPS) {
     // ---- epilogue: warp w reads TMEM lanes 32 (w % 4) .. of this CTA's 128 activation rows, one half of the weight rows
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     constexpr int HALF = NW / 2;
     const int quad = warp & 3, side = warp >> 2;
-    float* mine = turn + warp * (TURN_BYTES / 4);
-    int k = 0;  // blocks of K so far, over all tiles
-    bool alive = true;
-    pdl_wait();
-    for (int item = pair; item < items && alive; item += npairs) {
+    // with two parts the sides have accumulators of their own
+    const uint32_t part = P::PARTS == 2 ? side : 0, freed = cluster_addr(acc_free, 0);
+    uint32_t k = 0;  // blocks of K so far, over all tiles
+    int m_first = 0, n_first = 0;
+    const float *sx = nullptr, *sw = nullptr;
+    float fx = 0.f, fw = 0.f;  // scales of the next block
+    auto begin = [&](int item) {
       int mt, nt;
       split(item, mt, nt);
-      const int m_first = mt * 256 + rank * 128 + quad * 32, n_first = nt * NW + side * HALF;
-      const float* sx = a.sx + (size_t)min(m_first + lane, a.out.m - 1) * a.kblocks;
-      const float* sw = a.sw + (size_t)min(n_first / F8_BLOCK, (a.out.n - 1) / F8_BLOCK) * a.kblocks;
+      m_first = mt * 256 + rank * 128 + quad * 32;
+      n_first = nt * NW + side * HALF;
+      sx = a.sx + (size_t)min(m_first + lane, a.out.m - 1) * a.kblocks;
+      sw = a.sw + (size_t)min(n_first / F8_BLOCK, (a.out.n - 1) / F8_BLOCK) * a.kblocks;
+      fx = sx[0];
+      fw = sw[0];
+    };
+    pdl_wait();
+    begin(pair);
+    for (int item = pair; item < items; item += npairs) {
+      bool alive = true;
       float2 acc[HALF / 2];
 #pragma unroll
       for (int i = 0; i < HALF / 2; ++i) acc[i] = make_float2(0.f, 0.f);
-      float s = sx[0] * sw[0];
 #pragma unroll 1
       for (int kb = 0; kb < a.kblocks; ++kb, ++k) {
-        const int buf = k & 1;
-        const float now = s;
-        if (kb + 1 < a.kblocks) s = sx[kb + 1] * sw[kb + 1];  // in flight beside the wait
-        if (!(alive = w_wait(acc_full + 8 * buf, (uint32_t)((k >> 1) & 1), dead, a.status))) break;
+        const uint32_t buf = k % P::BUFS * P::PARTS + part;
+        if (!(alive = f_wait(acc_full + 8 * buf, k / P::BUFS & 1, dead, a.status))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t tl = tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(buf * NW + side * HALF);
-        uint32_t v[2][16];
+        const uint32_t tl = tmem + ((uint32_t)(32 * quad) << 16) + buf * 128 + (P::PARTS == 2 ? 0 : side * HALF);
+        const float2 f = make_float2(fx * fw, fx * fw);
+        fx = sx[min(kb + 1, a.kblocks - 1)];  // in flight until the next block
+        fw = sw[min(kb + 1, a.kblocks - 1)];
+        uint32_t v[4][16];
         x_ld16(tl, v[0]);
+        x_ld16(tl + 16, v[1]);
 #pragma unroll
-        for (int c = 0; c < HALF / 16; ++c) {
+        for (int c = 0; c < HALF / 32; ++c) {
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-          if (c + 1 < HALF / 16) x_ld16(tl + 16 * (c + 1), v[(c + 1) & 1]);
-          else {
+          if (c + 1 < HALF / 32) {
+            x_ld16(tl + 32 * (c + 1), v[2 * (c + 1) & 3]);
+            x_ld16(tl + 32 * (c + 1) + 16, v[(2 * (c + 1) & 3) + 1]);
+          } else {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) cluster_arrive(acc_free + 8 * buf, 0);
+            w_cluster_arrive(freed + 8 * buf);
           }
-          const float2 ss = make_float2(now, now);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            acc[8 * c + i] = fma2(make_float2(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])), ss, acc[8 * c + i]);
+          for (int i = 0; i < 16; ++i) {
+            const uint32_t* p = &v[(2 * c & 3) + i / 8][2 * i % 16];
+            acc[16 * c + i] = fma2(make_float2(__uint_as_float(p[0]), __uint_as_float(p[1])), f, acc[16 * c + i]);
+          }
         }
       }
       if (!alive) break;
-      // out, 16 columns at a time, turned in shared memory so that a row's columns leave together
-#pragma unroll
-      for (int c = 0; c < HALF / 16; ++c) {
-        if (n_first + 16 * c >= a.out.n) break;
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<float4*>(mine + lane * TURN_ROW + 4 * i) =
-              make_float4(acc[8 * c + 2 * i].x, acc[8 * c + 2 * i].y, acc[8 * c + 2 * i + 1].x, acc[8 * c + 2 * i + 1].y);
-        __syncwarp();
-        const int n = n_first + 16 * c + 4 * (lane & 3);
-#pragma unroll 1
-        for (int r = lane >> 2; r < 32 && m_first + r < a.out.m; r += 8) {
-          const float4 v = *reinterpret_cast<const float4*>(mine + r * TURN_ROW + 4 * (lane & 3));
-          if (a.vec) {  // whole fours: n is a multiple of four then
-            if (n < a.out.n) f8_put4(a.out, v, m_first + r, n);
-          } else {
-            const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (n + i < a.out.n) f8_put(a.out, e[i], m_first + r, n + i);
-          }
-        }
-      }
+      const int m_done = m_first, n_done = n_first;
+      if (item + npairs < items) begin(item + npairs);  // its first scales arrive meanwhile
+      f8_store_rows<HALF>(a, acc, turn + warp * TURN_BYTES, m_done, n_done);
     }
   } else if (warp == PAIR_EPI_WARPS) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     // ---- copy requester: a stage is one block of K, 128 activation rows and NW / 2 weight rows per CTA; the copies of both CTAs are
     // counted on the even CTA's barrier
     if (lane == 0) {
@@ -407,14 +463,15 @@ f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const
       for (int item = pair; item < items && alive; item += npairs) {
         int mt, nt;
         split(item, mt, nt);
-        const int xr = mt * 256 + rank * 128, wr = nt * NW + rank * (NW / 2);
+        const int xr = mt * 256 + rank * 128, wr = nt * NW + rank * 64;  // of every 128 columns of a product a CTA holds 64 weight rows
         for (int kb = 0; kb < a.kblocks; ++kb, ++k) {
           const int s = k % P::STAGES, round = k / P::STAGES;
           if (round > 0 && !(alive = x_wait(stage_free + 8 * s, (uint32_t)((round - 1) & 1), dead, a.status))) break;
           const uint32_t dst = smem_u32(sm + s * P::STAGE), bar = cluster_addr(full + 8 * s, 0);
           if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * P::STAGE);
           pair_tma_box2(dst, &xmap, kb * F8_BLOCK, xr, bar);
-          pair_tma_box2(dst + F8_A_BYTES, &wmap, kb * F8_BLOCK, wr, bar);
+#pragma unroll
+          for (int p = 0; p < P::PARTS; ++p) pair_tma_box2(dst + F8_A_BYTES + p * 64 * 128, &wmap, kb * F8_BLOCK, wr + 128 * p, bar);
         }
       }
       if (*dead) {
@@ -425,29 +482,31 @@ f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const
           for (int i = max(0, k - P::STAGES); i < k; ++i) x_drain(full + 8 * (i % P::STAGES), (uint32_t)((i / P::STAGES) & 1));
       }
     }
-  } else {
-    // ---- MMA issuer (even CTA): a block of K per accumulator; the next stage's barrier is polled before this one's MMAs are issued
-    int s = 0, k = 0;
-    uint32_t parity = 0, ready = 0;
-    bool alive = rank == 0;
-    const uint64_t adesc0 = x_desc_rows(smem_u32(sm)), bdesc0 = x_desc_rows(smem_u32(sm) + F8_A_BYTES);
-    for (int item = pair; item < items && alive; item += npairs) {
-      for (int kb = 0; kb < a.kblocks && alive; ++kb, ++k) {
-        const int buf = k & 1;
-        if (!__all_sync(0xFFFFFFFFu, ready) && !(alive = w_wait(full + 8 * s, parity, dead, a.status))) break;
-        if (k >= 2 && !(alive = w_wait(acc_free + 8 * buf, (uint32_t)(((k >> 1) - 1) & 1), dead, a.status))) break;
-        const int now = s;
-        if (++s == P::STAGES) { s = 0; parity ^= 1u; }
-        ready = x_poll(full + 8 * s, parity);
+  } else if (warp <= PAIR_EPI_WARPS + 2) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    // ---- two MMA issuers (even CTA), an accumulator of 128 weight rows and a block of K at a time: of the two parts of a block one each,
+    // or every other block. (One warp needs 460 cycles for an accumulator's waits, MMAs and commits, nearly twice what the MMAs take.)
+    const uint32_t which = warp - PAIR_EPI_WARPS - 1, part = P::PARTS == 2 ? which : 0, step = 2 / P::PARTS;
+    const uint32_t blocks = (uint32_t)((items - pair + npairs - 1) / npairs) * (uint32_t)a.kblocks;
+    if (rank == 0) {
+      const uint64_t adesc0 = x_desc_rows(smem_u32(sm)), bdesc0 = x_desc_rows(smem_u32(sm) + F8_A_BYTES) + part * (64 * 128 >> 4);
+      uint32_t s = P::PARTS == 2 ? 0 : which, parity = 0;
+      for (uint32_t k = s; k < blocks; k += step) {
+        const uint32_t buf = k % P::BUFS * P::PARTS + part;
+        if (!f_wait(full + 8 * s, parity, dead, a.status)) break;
+        if (k >= P::BUFS && !f_wait(acc_free + 8 * buf, (k / P::BUFS - 1) & 1, dead, a.status)) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint64_t at = (uint64_t)((now * P::STAGE) >> 4);
-        pair_mma4_f8<2>(tmem + (uint32_t)(buf * NW), adesc0 + at, bdesc0 + at, P::IDESC, 0u);
-        pair_commit(stage_free + 8 * now);
+        const uint64_t at = (uint64_t)((s * P::STAGE) >> 4);
+        pair_mma4_f8<2>(tmem + buf * 128, adesc0 + at, bdesc0 + at, P::IDESC, 0u);
         pair_commit(acc_full + 8 * buf);
+        pair_commit(stage_free + 8 * s);
+        if ((s += step) >= P::STAGES) { s -= P::STAGES; parity ^= 1u; }
       }
+      pair_commit(drained);
     }
-    if (rank == 0) pair_commit(drained);
     x_drain(drained, 0);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   }
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -514,17 +573,18 @@ int launch_pair(fb200_device* dev, const F8Job& j) {
   CUtensorMap xmap;
   if (!fb200_make_map_2d_bytes(&xmap, j.x, j.w->k, (uint64_t)j.out.m, j.ld, 128))
     return fb200_fail(dev, FB200_ERR_CUDA, "f8_mat_mul: tensor map refused (x %d rows every %zu bytes)", j.out.m, j.ld);
-  PairArgs a = {j.sx, j.w->scales, j.out, j.kblocks, (j.out.m + 255) / 256, (j.out.n + NW - 1) / NW, 1, 0, dev->status};
+  PairArgs a = {j.sx, j.w->scales, j.out, j.kblocks, (j.out.m + 255) / 256, (j.out.n + NW - 1) / NW, 1, 0, 0, dev->status};
   const long long items = (long long)a.m_tiles * a.n_tiles;
   if (items > 0x3FFFFFFF) return fb200_fail(dev, FB200_ERR_INVALID_SHAPE, "f8_mat_mul: %d x %d outputs are too many", j.out.m, j.out.n);
   // the activation rows of a group take at most 32 MB of L2
   const long long fit = (32ll << 20) / (256ll * F8_BLOCK * j.kblocks);
   a.m_group = fit < 1 ? 1 : fit > a.m_tiles ? a.m_tiles : (int)fit;
   const uintptr_t four = j.out.type == FB200_F32 ? 16 : 8;
+  a.pack = j.out.type != FB200_F32 && !j.out.bias && !j.out.r1 && !j.out.r2 && j.out.n % 8 == 0 && (uintptr_t)j.out.y % 16 == 0;
   a.vec = j.out.n % 4 == 0 && (uintptr_t)j.out.y % four == 0 && (uintptr_t)j.out.r1 % 16 == 0 && (uintptr_t)j.out.r2 % 16 == 0;
   const int pairs = items < dev->sm_count / 2 ? (int)items : dev->sm_count / 2;
   return fb200_launch(dev, f8_pair_kernel<NW>, dim3((unsigned)(2 * pairs)), dim3(PAIR_THREADS), (size_t)P::SMEM, true, a,
-                      NW == 256 ? j.w->map128 : j.w->map64, xmap);
+                      j.w->map64, xmap);
 }
 
 int f8_product(fb200_device* dev, const F8Job& j) {
