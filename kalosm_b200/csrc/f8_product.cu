@@ -58,22 +58,22 @@ __device__ __forceinline__ void f8_put(const F8Out& o, float v, int m, int n) {
 
 // ---- few activation rows ------------------------------------------------------------------------------------------------
 
-constexpr int FEW_SCALES = 16;  // blocks of K whose scales are fetched together
-
 template <int BM>
 struct Few {
-  static constexpr int EPI_WARPS = BM >= 64 ? 8 : 4, THREADS = (EPI_WARPS + 2) * 32;
+  static constexpr bool WIDE = BM >= 128;  // a CTA fills an SM: the copy requester's warpgroup hands registers to the epilogue's two
+  static constexpr int EPI_WARPS = BM >= 64 ? 8 : 4, THREADS = (EPI_WARPS + (WIDE ? 4 : 2)) * 32;
   static constexpr int COLS = BM * 4 / EPI_WARPS;  // activation rows of an epilogue thread
   static constexpr int STAGE = F8_A_BYTES + BM * 128;
-  // every stage of operands has an accumulator of its own, so that one arrival tells both rings that a block is multiplied
-  static constexpr int STAGES = BM == 16 ? 6 : BM == 32 ? 5 : 4;
-  static constexpr int TMEM = BM == 16 ? 128 : BM == 32 ? 256 : STAGES * BM;
-  static constexpr int SCALE_ROW = BM + 4, SCALE_BYTES = 2 * FEW_SCALES * SCALE_ROW * 4;
-  static constexpr int SMEM = STAGES * STAGE + SCALE_BYTES + 256 + 1024;
-  static constexpr int PER_SM = BM <= 64 ? 2 : 1;
+  static constexpr int STAGES = BM == 16 ? 5 : BM == 128 ? 6 : 4, BUFS = BM == 256 ? 2 : 4, TMEM = BUFS * BM;
+  static constexpr int AHEAD = BM == 256 ? 8 : 16;  // blocks of K whose scales are fetched together
+  static constexpr int SCALE_ROW = BM + 4, SCALE_BYTES = 2 * AHEAD * SCALE_ROW * 4;
+  // the partial sums that come in from the cluster: in a place of their own, or (larger ones) in the operands' when all are done with them
+  static constexpr int PART = BM * 128 * 4, PART_BYTES = BM <= 32 ? PART : 0;
+  static constexpr int SMEM = STAGES * STAGE + PART_BYTES + SCALE_BYTES + 256 + 1024;
+  static constexpr int PER_SM = WIDE ? 1 : 2;
   // instruction descriptor: f32 accumulator, e4m3 A and B, both K-major, N = BM, M = 128
   static constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(BM >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-  static_assert(STAGES * STAGE >= BM * 128 * 4, "the partial sums take the operands' place");
+  static_assert(PART_BYTES || STAGES * STAGE >= PART, "the partial sums take the operands' place");
 };
 
 struct FewArgs {
@@ -83,10 +83,14 @@ struct FewArgs {
   int* status;
 };
 
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
+// Stores into the shared memory of a CTA of the cluster, counted in bytes on a barrier there
+__device__ __forceinline__ void st_cluster4(uint32_t addr, float2 a, float2 b, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];"
+               ::"r"(addr), "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void st_cluster2(uint32_t addr, float2 a, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];"
+               ::"r"(addr), "f"(a.x), "f"(a.y), "r"(bar) : "memory");
 }
 
 template <int BM>
@@ -96,22 +100,35 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
   extern __shared__ uint8_t sm_raw[];
   // the same offset in every CTA of the cluster: their dynamic shared memory starts at the same address
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~(uintptr_t)1023);
-  float* scales = reinterpret_cast<float*>(sm + F::STAGES * F::STAGE);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + F::STAGES * F::STAGE + F::SCALE_BYTES);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * F::STAGES + 1);
+  float* part = reinterpret_cast<float*>(sm + (F::PART_BYTES ? F::STAGES * F::STAGE : 0));
+  float* scales = reinterpret_cast<float*>(sm + F::STAGES * F::STAGE + F::PART_BYTES);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + F::STAGES * F::STAGE + F::PART_BYTES + F::SCALE_BYTES);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * F::STAGES + 2 * F::BUFS + 2);
   volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const uint32_t full = smem_u32(bars), multiplied = full + 8 * F::STAGES, acc_free = multiplied + 8 * F::STAGES, drained = acc_free + 8 * F::STAGES;
+  const uint32_t full = smem_u32(bars), stage_free = full + 8 * F::STAGES, acc_full = stage_free + 8 * F::STAGES, acc_free = acc_full + 8 * F::BUFS,
+                 drained = acc_free + 8 * F::BUFS, joined = drained + 8;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = (int)cluster_rank(), tile = (int)blockIdx.x / a.split;
   // activation tiles fastest: the CTAs that run together share their weight rows in L2
   const int nt = tile / a.m_tiles, mt = tile - nt * a.m_tiles, m0 = mt * BM;
   const int kb0 = (int)((long long)a.kblocks * rank / a.split), nkb = (int)((long long)a.kblocks * (rank + 1) / a.split) - kb0;
+  const int pre = min(F::STAGES, nkb);
 
-  if (tid == 0) {
+  // The copy requester sets the barriers up and asks for the first weights, which depend on no kernel in front, while tensor memory is
+  // allocated (1650 cycles to that point, and the weights' latency after it, when it was done before)
+  if (tid == F::EPI_WARPS * 32) {
     *dead = 0;
-    for (int i = 0; i < F::STAGES; ++i) { mbar_init(full + 8 * i, 1); mbar_init(multiplied + 8 * i, 1); mbar_init(acc_free + 8 * i, F::EPI_WARPS); }
+    for (int i = 0; i < F::STAGES; ++i) { mbar_init(full + 8 * i, 1); mbar_init(stage_free + 8 * i, 1); }
+    for (int i = 0; i < F::BUFS; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_free + 8 * i, F::EPI_WARPS); }
     mbar_init(drained, 1);
+    mbar_init(joined, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    mbar_expect_tx(joined, a.split > 1 ? F::PART : 0);
+    for (int i = 0; i < pre; ++i) {
+      mbar_expect_tx(full + 8 * i, F::STAGE);
+      x_tma_box2(smem_u32(sm + i * F::STAGE), &wmap, (kb0 + i) * F8_BLOCK, nt * 128, full + 8 * i);
+    }
   }
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(F::TMEM) : "memory");
@@ -122,79 +139,133 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
   pdl_launch_dependents_small();  // behind the allocation: a dependent must not take columns that this grid still waits for
+  // the first meeting of the cluster: everybody's place for partial sums may be written
+  if (F::PART_BYTES && a.split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 
-  float2 acc[F::COLS / 2];
-#pragma unroll
-  for (int i = 0; i < F::COLS / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+  // The cluster meets twice before anybody's sums are complete (warps come from their roles): everybody's place for partial sums may be
+  // written, and everybody has sent, so that nobody leaves while something may still come
+  auto place_free = [&]() {
+    if (!F::PART_BYTES) {
+      __syncthreads();  // nobody here multiplies from the operands any more
+      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    }
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  };
 
   if (warp < F::EPI_WARPS) {
+    if (F::WIDE) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     // ---- epilogue: warp w reads TMEM lanes 32 (w % 4) .. = weight rows, COLS of the activation rows
     const int quad = warp & 3, col0 = (warp >> 2) * F::COLS;
-    constexpr int ET = F::EPI_WARPS * 32, MINE = FEW_SCALES * BM / ET;
+    constexpr int ET = F::EPI_WARPS * 32, MINE = F::AHEAD * BM / ET, CHUNK = F::COLS < 32 ? F::COLS : 32;
+    float2 acc[F::COLS / 2];
+#pragma unroll
+    for (int i = 0; i < F::COLS / 2; ++i) acc[i] = make_float2(0.f, 0.f);
     float ahead[MINE];
-    // scales of FEW_SCALES blocks: thread t holds block t % 16 of activation rows t / 16, ..
+    // scales of AHEAD blocks: thread t holds block t % AHEAD of activation rows t / AHEAD, ..
     auto fetch = [&](int first) {
-      const int kb = kb0 + first + (tid % FEW_SCALES);
-      const bool in = first + (tid % FEW_SCALES) < nkb;
+      const int kb = kb0 + first + (tid % F::AHEAD);
+      const bool in = first + (tid % F::AHEAD) < nkb;
       const float w = in ? a.sw[(size_t)nt * a.kblocks + kb] : 0.f;
 #pragma unroll
       for (int i = 0; i < MINE; ++i) {
-        const int m = m0 + tid / FEW_SCALES + i * (ET / FEW_SCALES);
+        const int m = m0 + tid / F::AHEAD + i * (ET / F::AHEAD);
         ahead[i] = in && m < a.out.m ? a.sx[(size_t)m * a.kblocks + kb] * w : 0.f;
       }
     };
     pdl_wait();
     fetch(0);
-    int st = 0;
+    int buf = 0;
     uint32_t parity = 0;
     for (int i = 0; i < nkb; ++i) {
-      const int at = i % FEW_SCALES;
+      const int at = i % F::AHEAD;
+      const float* half = scales + ((i / F::AHEAD) & 1) * F::AHEAD * F::SCALE_ROW;
       if (at == 0) {
         // the other half was last read before everybody came to this barrier's predecessor
-        float* half = scales + ((i / FEW_SCALES) & 1) * FEW_SCALES * F::SCALE_ROW;
 #pragma unroll
-        for (int j = 0; j < MINE; ++j) half[(tid % FEW_SCALES) * F::SCALE_ROW + tid / FEW_SCALES + j * (ET / FEW_SCALES)] = ahead[j];
+        for (int j = 0; j < MINE; ++j) const_cast<float*>(half)[(tid % F::AHEAD) * F::SCALE_ROW + tid / F::AHEAD + j * (ET / F::AHEAD)] = ahead[j];
         asm volatile("bar.sync 1, %0;" ::"n"(ET) : "memory");
-        if (i + FEW_SCALES < nkb) fetch(i + FEW_SCALES);
+        if (i + F::AHEAD < nkb) fetch(i + F::AHEAD);
       }
-      if (!f_wait(multiplied + 8 * st, parity, dead, a.status)) {
+      if (!f_wait(acc_full + 8 * buf, parity, dead, a.status)) {
         // the barriers of the scales to come are met all the same
-        for (int j = (i / FEW_SCALES + 1) * FEW_SCALES; j < nkb; j += FEW_SCALES) asm volatile("bar.sync 1, %0;" ::"n"(ET) : "memory");
+        for (int j = (i / F::AHEAD + 1) * F::AHEAD; j < nkb; j += F::AHEAD) asm volatile("bar.sync 1, %0;" ::"n"(ET) : "memory");
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t tl = tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(st * BM + col0), freed = acc_free + 8 * st;
-      uint32_t v[F::COLS / 16][16];
+      const uint32_t tl = tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(buf * BM + col0), freed = acc_free + 8 * buf;
+      const float4* sc = reinterpret_cast<const float4*>(half + at * F::SCALE_ROW + col0);
+      uint32_t v[2 * CHUNK / 16][16];
 #pragma unroll
-      for (int j = 0; j < F::COLS / 16; ++j) x_ld16(tl + 16 * j, v[j]);
-      if (++st == F::STAGES) { st = 0; parity ^= 1u; }
-      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      w_arrive(freed);
-      const float4* sc = reinterpret_cast<const float4*>(scales + (((i / FEW_SCALES) & 1) * FEW_SCALES + at) * F::SCALE_ROW + col0);
+      for (int j = 0; j < CHUNK / 16; ++j) x_ld16(tl + 16 * j, v[j]);
 #pragma unroll
-      for (int j = 0; j < F::COLS / 4; ++j) {
-        const float4 f = sc[j];
-        const uint32_t* p = &v[j / 4][4 * (j % 4)];
-        acc[2 * j] = fma2(make_float2(__uint_as_float(p[0]), __uint_as_float(p[1])), make_float2(f.x, f.y), acc[2 * j]);
-        acc[2 * j + 1] = fma2(make_float2(__uint_as_float(p[2]), __uint_as_float(p[3])), make_float2(f.z, f.w), acc[2 * j + 1]);
+      for (int c = 0; c < F::COLS / CHUNK; ++c) {
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (c + 1 < F::COLS / CHUNK) {
+#pragma unroll
+          for (int j = 0; j < CHUNK / 16; ++j) x_ld16(tl + CHUNK * (c + 1) + 16 * j, v[((c + 1) & 1) * (CHUNK / 16) + j]);
+        } else {
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          w_arrive(freed);
+        }
+#pragma unroll
+        for (int j = 0; j < CHUNK / 4; ++j) {
+          const float4 f = sc[c * (CHUNK / 4) + j];
+          const uint32_t* p = &v[(c & 1) * (CHUNK / 16) + j / 4][4 * (j % 4)];
+          float2* to = acc + c * (CHUNK / 2) + 2 * j;
+          to[0] = fma2(make_float2(__uint_as_float(p[0]), __uint_as_float(p[1])), make_float2(f.x, f.y), to[0]);
+          to[1] = fma2(make_float2(__uint_as_float(p[2]), __uint_as_float(p[3])), make_float2(f.z, f.w), to[1]);
+        }
       }
+      if (++buf == F::BUFS) { buf = 0; parity ^= 1u; }
+    }
+    const int row = 32 * quad + lane, n = nt * 128 + row;
+    if (a.split == 1) {
+      if (n < a.out.n)
+#pragma unroll
+        for (int j = 0; j < F::COLS; ++j)
+          if (m0 + col0 + j < a.out.m) f8_put(a.out, j & 1 ? acc[j / 2].y : acc[j / 2].x, m0 + col0 + j, n);
+    } else {
+      // the sums of the cluster's ranges of K: rank q gets activation rows BM q / split .. of all, [rank][weight row][activation row], and
+      // adds them in the order of the ranks
+      const int per = BM / a.split;
+      const uint32_t mine = smem_u32(part) + (uint32_t)((rank * 128 + row) * per) * 4;
+      __syncwarp();
+      place_free();
+      if (per >= 4) {
+#pragma unroll
+        for (int j = 0; j < F::COLS; j += 4) {
+          const int to = (col0 + j) / per;
+          st_cluster4(cluster_addr(mine + (uint32_t)(col0 + j - to * per) * 4, to), acc[j / 2], acc[j / 2 + 1], cluster_addr(joined, to));
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < F::COLS; j += 2) st_cluster2(cluster_addr(mine, (col0 + j) / 2), acc[j / 2], cluster_addr(joined, (col0 + j) / 2));
+      }
+      __syncwarp();
+      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+      if (f_wait(joined, 0, dead, a.status)) {
+        for (int j = warp >> 2; j < per && m0 + rank * per + j < a.out.m; j += F::EPI_WARPS / 4) {
+          const float* from = part + row * per + j;
+          float v = 0.f;
+          for (int q = 0; q < a.split; ++q) v += from[q * 128 * per];
+          if (n < a.out.n) f8_put(a.out, v, m0 + rank * per + j, n);
+        }
+      }
+      __syncwarp();
+      asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+      if (*dead) x_drain(joined, 0);
     }
   } else if (warp == F::EPI_WARPS) {
-    // ---- copy requester; the weights do not depend on the kernel in front
+    if (F::WIDE) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    // ---- copy requester, from the first activation rows on
     if (lane == 0) {
-      const int pre = min(F::STAGES, nkb);
-      for (int i = 0; i < pre; ++i) {
-        mbar_expect_tx(full + 8 * i, F::STAGE);
-        x_tma_box2(smem_u32(sm + i * F::STAGE), &wmap, (kb0 + i) * F8_BLOCK, nt * 128, full + 8 * i);
-      }
       pdl_wait();
       int i = 0;
       for (; i < pre; ++i) x_tma_box2(smem_u32(sm + i * F::STAGE + F8_A_BYTES), &xmap, (kb0 + i) * F8_BLOCK, m0, full + 8 * i);
       for (; i < nkb; ++i) {
         const int s = i % F::STAGES;
-        if (!x_wait(multiplied + 8 * s, (uint32_t)((i / F::STAGES - 1) & 1), dead, a.status)) break;
+        if (!x_wait(stage_free + 8 * s, (uint32_t)((i / F::STAGES - 1) & 1), dead, a.status)) break;
         const uint32_t dst = smem_u32(sm + s * F::STAGE), bar = full + 8 * s;
         mbar_expect_tx(bar, F::STAGE);
         x_tma_box2(dst, &wmap, (kb0 + i) * F8_BLOCK, nt * 128, bar);
@@ -204,52 +275,34 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
         for (int j = max(0, i - F::STAGES); j < i; ++j) x_drain(full + 8 * (j % F::STAGES), (uint32_t)((j / F::STAGES) & 1));
     }
   } else {
-    // ---- MMA issuer; the next block's barriers are polled before this one's MMAs are issued
-    const uint64_t adesc0 = x_desc_rows(smem_u32(sm)), bdesc0 = x_desc_rows(smem_u32(sm) + F8_A_BYTES);
-    int st = 0;
-    uint32_t parity = 0, ready = 0, room = 1;  // a buffer's first use waits for nobody
-    for (int i = 0; i < nkb; ++i) {
-      if (!__all_sync(0xFFFFFFFFu, room) && !f_wait(acc_free + 8 * st, parity ^ 1u, dead, a.status)) break;
-      if (!__all_sync(0xFFFFFFFFu, ready) && !f_wait(full + 8 * st, parity, dead, a.status)) break;
-      const int now = st;
-      if (++st == F::STAGES) { st = 0; parity ^= 1u; }
-      ready = x_poll(full + 8 * st, parity);
-      room = i + 1 < F::STAGES ? 1u : x_poll(acc_free + 8 * st, parity ^ 1u);
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint64_t at = (uint64_t)((now * F::STAGE) >> 4);
-      w_mma4_f8<2, 2>(tmem + (uint32_t)(now * BM), adesc0 + at, bdesc0 + at, F::IDESC, 0u);
-      w_commit(multiplied + 8 * now);
+    if (F::WIDE) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == F::EPI_WARPS + 1) {
+      // ---- MMA issuer
+      const uint64_t adesc0 = x_desc_rows(smem_u32(sm)), bdesc0 = x_desc_rows(smem_u32(sm) + F8_A_BYTES);
+      int st = 0, buf = 0;
+      uint32_t parity = 0, round = 0;
+      for (int i = 0; i < nkb; ++i) {
+        if (!f_wait(full + 8 * st, parity, dead, a.status)) break;
+        if (round && !f_wait(acc_free + 8 * buf, (round - 1) & 1, dead, a.status)) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t at = (uint64_t)((st * F::STAGE) >> 4);
+        w_mma4_f8<2, 2>(tmem + (uint32_t)(buf * BM), adesc0 + at, bdesc0 + at, F::IDESC, 0u);
+        w_commit(acc_full + 8 * buf);
+        w_commit(stage_free + 8 * st);
+        if (++st == F::STAGES) { st = 0; parity ^= 1u; }
+        if (++buf == F::BUFS) { buf = 0; ++round; }
+      }
+      w_commit(drained);
+      x_drain(drained, 0);
     }
-    w_commit(drained);
-    x_drain(drained, 0);
+  }
+  if (warp >= F::EPI_WARPS && a.split > 1) {
+    __syncwarp();
+    place_free();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
   __syncwarp();
-
-  // ---- the sums of the cluster's ranges of K, joined in the order of the ranks
-  const int quad = warp & 3, col0 = (warp >> 2) * F::COLS, n = nt * 128 + 32 * quad + lane;
-  if (a.split == 1) {
-    if (warp < F::EPI_WARPS && n < a.out.n)
-#pragma unroll
-      for (int j = 0; j < F::COLS; ++j)
-        if (m0 + col0 + j < a.out.m) f8_put(a.out, j & 1 ? acc[j / 2].y : acc[j / 2].x, m0 + col0 + j, n);
-  } else {
-    __syncthreads();  // nobody multiplies from the operands any more
-    float* part = reinterpret_cast<float*>(sm);
-    if (warp < F::EPI_WARPS)
-#pragma unroll
-      for (int j = 0; j < F::COLS; ++j) part[(col0 + j) * 128 + 32 * quad + lane] = j & 1 ? acc[j / 2].y : acc[j / 2].x;
-    cluster_sync();
-    if (warp < F::EPI_WARPS && n < a.out.n) {
-      const int per = BM / a.split;
-      for (int j = rank * per + (warp >> 2); j < (rank + 1) * per && m0 + j < a.out.m; j += F::EPI_WARPS / 4) {
-        const uint32_t mine = smem_u32(part + j * 128 + 32 * quad + lane);
-        float v = 0.f;
-        for (int q = 0; q < a.split; ++q) v += ld_cluster(cluster_addr(mine, (uint32_t)q));
-        f8_put(a.out, v, m0 + j, n);
-      }
-    }
-    cluster_sync();  // the others may still read
-  }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(F::TMEM) : "memory");
@@ -589,22 +642,28 @@ int launch_pair(fb200_device* dev, const F8Job& j) {
 
 int f8_product(fb200_device* dev, const F8Job& j) {
   const int m = j.out.m, n_tiles = (j.out.n + 127) / 128;
-  int bm = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128, split = 1;
+  int bm = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256, split = 1, pair = 0;
   const int tiles = n_tiles * ((m + bm - 1) / bm);
   while (split < 8 && tiles * split * 2 <= dev->sm_count * (bm <= 64 ? 2 : 1) && j.kblocks >= split * 4) split *= 2;
-  if (m > 256) bm = 256, split = 2;
-  // FB200_F8_TILE="BM,SPLIT": activation rows and ranges of K of the kernel for few rows; "256,1" / "256,2": pairs with 128 / 256 weight
-  // rows (tests, tuning; read per call)
-  int fbm, fsplit;
-  if (const char* cfg = getenv("FB200_F8_TILE"))
-    if (sscanf(cfg, "%d,%d", &fbm, &fsplit) == 2) bm = fbm, split = fsplit;
-  if (split != 1 && split != 2 && split != 4 && split != 8) split = 1;
+  if (m > 256) pair = 256;
+  // FB200_F8_TILE (tests, tuning; read per call): "BM,SPLIT" activation rows and ranges of K of the kernel for few rows, "pair,NW" pairs
+  // with 128 or 256 weight rows; what there is not leaves the choice to the rule
+  if (const char* cfg = getenv("FB200_F8_TILE")) {
+    int fbm, fsplit;
+    if (sscanf(cfg, "pair,%d", &fbm) == 1) {
+      if (fbm == 128 || fbm == 256) pair = fbm;
+    } else if (sscanf(cfg, "%d,%d", &fbm, &fsplit) == 2 && (fbm == 16 || fbm == 32 || fbm == 64 || fbm == 128 || fbm == 256) &&
+               (fsplit == 1 || fsplit == 2 || fsplit == 4 || fsplit == 8)) {
+      bm = fbm, split = fsplit, pair = 0;
+    }
+  }
+  if (pair) return pair == 128 ? launch_pair<128>(dev, j) : launch_pair<256>(dev, j);
   switch (bm) {
     case 16: return launch_few<16>(dev, j, split);
     case 32: return launch_few<32>(dev, j, split);
     case 64: return launch_few<64>(dev, j, split);
     case 128: return launch_few<128>(dev, j, split);
-    default: return split == 1 ? launch_pair<128>(dev, j) : launch_pair<256>(dev, j);
+    default: return launch_few<256>(dev, j, split);
   }
 }
 
