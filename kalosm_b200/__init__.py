@@ -455,17 +455,18 @@ class Device:
                     sum_out: Tensor = None, out: "F8Rows" = None) -> "F8Rows":
         """RMSNorm of x (+ residual) as rows of 8 bits; `sum_out` receives x + residual and may be x or residual itself."""
         kind, rows, n = _f8_input(self, "x", x)
-        for name, t in (("residual", residual), ("sum_out", sum_out)):
-            if t is not None and (t.nbytes != x.nbytes or t.dtype != x.dtype or t.device is not self):
-                raise FusorError(ERR_INVALID_SHAPE, f"{name} must be a tensor like x")
+        rp = sp = bp = None
+        if residual is not None:
+            rp = _f8_like(x, "residual", residual)
+        if sum_out is not None:
+            sp = _f8_like(x, "sum_out", sum_out)
         x._require_f32("weight", weight, n)
-        x._require_f32("bias", bias, n)
+        if bias is not None:
+            x._require_f32("bias", bias, n)
+            bp = bias.ptr
         out = _f8_output(self, out, x.shape)
-        self._check(self.lib.fb200_rms_norm_f8(self.h, x.ptr, n, residual.ptr if residual is not None else None, n,
-                                               sum_out.ptr if sum_out is not None else None, n, kind,
-                                               weight.ptr if weight is not None else None,
-                                               bias.ptr if bias is not None else None, eps, rows, n, out.codes.ptr, out.ld,
-                                               out.scales.ptr))
+        self._check(self.lib.fb200_rms_norm_f8(self.h, x.ptr, n, rp, n, sp, n, kind, weight.ptr if weight is not None else None, bp,
+                                               eps, rows, n, out.codes.ptr, out.ld, out.scales.ptr))
         return out
 
     def close(self) -> None:
@@ -562,10 +563,16 @@ def _f8_input(device: Device, name: str, x: Tensor):
     return kind, (x.nbytes // x.dtype.itemsize // n if n else 0), n
 
 
+def _f8_like(x: Tensor, name: str, t: Tensor) -> int:
+    if t.nbytes != x.nbytes or t.dtype != x.dtype or t.device is not x.device:
+        raise FusorError(ERR_INVALID_SHAPE, f"{name} must be a tensor like x")
+    return t.ptr
+
+
 def _f8_output(device: Device, out: Optional["F8Rows"], shape) -> "F8Rows":
     if out is None:
         return F8Rows(device, shape)
-    if out.shape[-1:] != shape[-1:] or out.rows != _rows_of(shape) or out.device is not device:
+    if out.shape != shape and (out.shape[-1:] != shape[-1:] or out.rows != _rows_of(shape)) or out.device is not device:
         raise FusorError(ERR_INVALID_SHAPE, f"out must hold rows of shape {tuple(shape)} on this device handle (got {out.shape})")
     return out
 

@@ -41,16 +41,12 @@ struct F8Out {
   int m, n;
 };
 
-__device__ __forceinline__ float f8_epilogue(const F8Out& o, float v, int m, int n) {
+// The output (m, n): v + its bias + the residuals, rounded once
+__device__ __forceinline__ void f8_put(const F8Out& o, float v, float bias, int m, int n) {
   const size_t at = (size_t)m * o.n + n;
-  if (o.bias) v += o.bias[n];
+  v += bias;
   if (o.r1) v += o.r1[at];
   if (o.r2) v += o.r2[at];
-  return v;
-}
-__device__ __forceinline__ void f8_put(const F8Out& o, float v, int m, int n) {
-  const size_t at = (size_t)m * o.n + n;
-  v = f8_epilogue(o, v, m, n);
   if (o.type == FB200_F32) reinterpret_cast<float*>(o.y)[at] = v;
   else if (o.type == FB200_BF16) reinterpret_cast<__nv_bfloat16*>(o.y)[at] = __float2bfloat16(v);
   else reinterpret_cast<__half*>(o.y)[at] = __float2half(v);
@@ -220,11 +216,12 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
       if (++buf == F::BUFS) { buf = 0; parity ^= 1u; }
     }
     const int row = 32 * quad + lane, n = nt * 128 + row;
+    const float bias = a.out.bias && n < a.out.n ? a.out.bias[n] : 0.f;
     if (a.split == 1) {
       if (n < a.out.n)
 #pragma unroll
         for (int j = 0; j < F::COLS; ++j)
-          if (m0 + col0 + j < a.out.m) f8_put(a.out, j & 1 ? acc[j / 2].y : acc[j / 2].x, m0 + col0 + j, n);
+          if (m0 + col0 + j < a.out.m) f8_put(a.out, j & 1 ? acc[j / 2].y : acc[j / 2].x, bias, m0 + col0 + j, n);
     } else {
       // the sums of the cluster's ranges of K: rank q gets activation rows BM q / split .. of all, [rank][weight row][activation row], and
       // adds them in the order of the ranks
@@ -249,7 +246,7 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
           const float* from = part + row * per + j;
           float v = 0.f;
           for (int q = 0; q < a.split; ++q) v += from[q * 128 * per];
-          if (n < a.out.n) f8_put(a.out, v, m0 + rank * per + j, n);
+          if (n < a.out.n) f8_put(a.out, v, bias, m0 + rank * per + j, n);
         }
       }
       __syncwarp();
@@ -339,9 +336,9 @@ __device__ __forceinline__ uint32_t f8_pair(const F8Out& o, float2 v) {
   return o.type == FB200_BF16 ? *reinterpret_cast<const uint32_t*>(&b) : *reinterpret_cast<const uint32_t*>(&h);
 }
 // Four neighbouring outputs
-__device__ __forceinline__ void f8_put4(const F8Out& o, float4 v, int m, int n) {
+__device__ __forceinline__ void f8_put4(const F8Out& o, float4 v, const float4& bias, int m, int n) {
   const size_t at = (size_t)m * o.n + n;
-  if (o.bias) { v.x += o.bias[n]; v.y += o.bias[n + 1]; v.z += o.bias[n + 2]; v.w += o.bias[n + 3]; }
+  v.x += bias.x; v.y += bias.y; v.z += bias.z; v.w += bias.w;
   if (o.r1) { const float4 r = *reinterpret_cast<const float4*>(o.r1 + at); v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w; }
   if (o.r2) { const float4 r = *reinterpret_cast<const float4*>(o.r2 + at); v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w; }
   if (o.type == FB200_F32) {
@@ -389,15 +386,19 @@ __device__ __forceinline__ void f8_store_rows(const PairArgs& a, const float2 (&
     }
     __syncwarp();
     if (a.vec) {  // whole fours: N is a multiple of four then
-#pragma unroll 2
-      for (int r = lane >> 3; r < 32 && r < m_end; r += 4)
-        if (32 * c + 4 * (lane & 7) < n_end)
-          f8_put4(a.out, *reinterpret_cast<const float4*>(turn + r * 128 + (((lane & 7) ^ (r & 7)) << 4)), m0 + r, n0 + 32 * c + 4 * (lane & 7));
+      const int n = n0 + 32 * c + 4 * (lane & 7);
+      if (n >= a.out.n) continue;
+      const float4 bias = a.out.bias ? make_float4(a.out.bias[n], a.out.bias[n + 1], a.out.bias[n + 2], a.out.bias[n + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int r = lane >> 3; r < min(32, m_end); r += 4)
+        f8_put4(a.out, *reinterpret_cast<const float4*>(turn + r * 128 + (((lane & 7) ^ (r & 7)) << 4)), bias, m0 + r, n);
     } else {
-#pragma unroll 2
-      for (int r = 0; r < 32 && r < m_end; ++r)
-        if (32 * c + lane < n_end)
-          f8_put(a.out, *reinterpret_cast<const float*>(turn + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3)), m0 + r, n0 + 32 * c + lane);
+      const int n = n0 + 32 * c + lane;
+      if (n >= a.out.n) continue;
+      const float bias = a.out.bias ? a.out.bias[n] : 0.f;
+#pragma unroll 8
+      for (int r = 0; r < min(32, m_end); ++r)
+        f8_put(a.out, *reinterpret_cast<const float*>(turn + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3)), bias, m0 + r, n);
     }
   }
 }
