@@ -39,6 +39,8 @@ struct F8Out {
   uint32_t type;
   const float *r1, *r2, *bias;
   int m, n;
+  int vec;   // four columns of y (and of the residuals) are aligned
+  int pack;  // 16-bit y without residual or bias, eight columns aligned: rounded before they are turned
 };
 
 // The output (m, n): v + its bias + the residuals, rounded once
@@ -52,24 +54,93 @@ __device__ __forceinline__ void f8_put(const F8Out& o, float v, float bias, int 
   else reinterpret_cast<__half*>(o.y)[at] = __float2half(v);
 }
 
+constexpr int TURN_BYTES = 32 * 128;  // a warp's 32 rows x 128 bytes on their way out, 16-byte piece p of row r at place p ^ (r % 8)
+
+__device__ __forceinline__ uint32_t f8_pair(const F8Out& o, float2 v) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(v.x, v.y);
+  const __half2 h = __floats2half2_rn(v.x, v.y);
+  return o.type == FB200_BF16 ? *reinterpret_cast<const uint32_t*>(&b) : *reinterpret_cast<const uint32_t*>(&h);
+}
+// Four neighbouring outputs
+__device__ __forceinline__ void f8_put4(const F8Out& o, float4 v, const float4& bias, int m, int n) {
+  const size_t at = (size_t)m * o.n + n;
+  v.x += bias.x; v.y += bias.y; v.z += bias.z; v.w += bias.w;
+  if (o.r1) { const float4 r = *reinterpret_cast<const float4*>(o.r1 + at); v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w; }
+  if (o.r2) { const float4 r = *reinterpret_cast<const float4*>(o.r2 + at); v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w; }
+  if (o.type == FB200_F32) {
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(o.y) + at) = v;
+  } else {
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(o.y) + at) = make_uint2(f8_pair(o, make_float2(v.x, v.y)), f8_pair(o, make_float2(v.z, v.w)));
+  }
+}
+
+// A warp's 32 rows from m0 on, COLS columns from n0 on, a row per thread, to y: turned in shared memory, so that a row's columns leave
+// together.
+template <int COLS>
+__device__ __forceinline__ void f8_store_rows(const F8Out& o, const float2 (&acc)[COLS / 2], uint8_t* turn, int m0, int n0) {
+  const int lane = threadIdx.x & 31, m_end = o.m - m0, n_end = o.n - n0;
+  if (o.pack) {
+    const uint8_t* from = turn + (lane >> 3) * 128;
+    uint16_t* to = reinterpret_cast<uint16_t*>(o.y) + (size_t)m0 * o.n + n0 + 8 * (lane & 7);
+#pragma unroll
+    for (int c = 0; c < COLS / 64; ++c) {
+      if (64 * c >= n_end) break;
+      __syncwarp();
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        const float2* v = acc + 32 * c + 4 * p;
+        *reinterpret_cast<uint4*>(turn + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_uint4(f8_pair(o, v[0]), f8_pair(o, v[1]), f8_pair(o, v[2]), f8_pair(o, v[3]));
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3);
+        const uint4 v = *reinterpret_cast<const uint4*>(from + 512 * i + (((lane & 7) ^ (r & 7)) << 4));
+        if (r < m_end && 64 * c + 8 * (lane & 7) < n_end) *reinterpret_cast<uint4*>(to + (size_t)r * o.n + 64 * c) = v;
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int c = 0; c < COLS / 32; ++c) {
+    if (32 * c >= n_end) break;
+    __syncwarp();
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      const float2* v = acc + 16 * c + 2 * p;
+      *reinterpret_cast<float4*>(turn + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+    }
+    __syncwarp();
+    if (o.vec) {  // whole fours: N is a multiple of four then
+      const int n = n0 + 32 * c + 4 * (lane & 7);
+      if (n >= o.n) continue;
+      const float4 bias = o.bias ? make_float4(o.bias[n], o.bias[n + 1], o.bias[n + 2], o.bias[n + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int r = lane >> 3; r < min(32, m_end); r += 4)
+        f8_put4(o, *reinterpret_cast<const float4*>(turn + r * 128 + (((lane & 7) ^ (r & 7)) << 4)), bias, m0 + r, n);
+    } else {
+      const int n = n0 + 32 * c + lane;
+      if (n >= o.n) continue;
+      const float bias = o.bias ? o.bias[n] : 0.f;
+#pragma unroll 8
+      for (int r = 0; r < min(32, m_end); ++r)
+        f8_put(o, *reinterpret_cast<const float*>(turn + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3)), bias, m0 + r, n);
+    }
+  }
+}
+
 // ---- few activation rows ------------------------------------------------------------------------------------------------
 
 template <int BM>
 struct Few {
-  static constexpr bool WIDE = BM >= 128;  // a CTA fills an SM: the copy requester's warpgroup hands registers to the epilogue's two
-  static constexpr int EPI_WARPS = BM >= 64 ? 8 : 4, THREADS = (EPI_WARPS + (WIDE ? 4 : 2)) * 32;
-  static constexpr int COLS = BM * 4 / EPI_WARPS;  // activation rows of an epilogue thread
-  static constexpr int STAGE = F8_A_BYTES + BM * 128;
-  static constexpr int STAGES = BM == 16 ? 5 : BM == 128 ? 6 : 4, BUFS = BM == 256 ? 2 : 4, TMEM = BUFS * BM;
-  static constexpr int AHEAD = BM == 256 ? 8 : 16;  // blocks of K whose scales are fetched together
+  static constexpr int EPI_WARPS = 4, THREADS = (EPI_WARPS + 2) * 32;
+  static constexpr int STAGE = F8_A_BYTES + BM * 128, STAGES = BM == 16 ? 5 : 4, BUFS = 4, TMEM = BUFS * BM;
+  static constexpr int AHEAD = 16;  // blocks of K whose scales are fetched together
   static constexpr int SCALE_ROW = BM + 4, SCALE_BYTES = 2 * AHEAD * SCALE_ROW * 4;
-  // the partial sums that come in from the cluster: in a place of their own, or (larger ones) in the operands' when all are done with them
-  static constexpr int PART = BM * 128 * 4, PART_BYTES = BM <= 32 ? PART : 0;
-  static constexpr int SMEM = STAGES * STAGE + PART_BYTES + SCALE_BYTES + 256 + 1024;
-  static constexpr int PER_SM = WIDE ? 1 : 2;
+  static constexpr int PART = BM * 128 * 4;  // the partial sums that come in from the cluster
+  static constexpr int SMEM = STAGES * STAGE + PART + SCALE_BYTES + 256 + 1024;  // two CTAs to an SM
   // instruction descriptor: f32 accumulator, e4m3 A and B, both K-major, N = BM, M = 128
   static constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(BM >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-  static_assert(PART_BYTES || STAGES * STAGE >= PART, "the partial sums take the operands' place");
 };
 
 struct FewArgs {
@@ -90,15 +161,15 @@ __device__ __forceinline__ void st_cluster2(uint32_t addr, float2 a, uint32_t ba
 }
 
 template <int BM>
-__global__ void __launch_bounds__(Few<BM>::THREADS, Few<BM>::PER_SM)
+__global__ void __launch_bounds__(Few<BM>::THREADS, 2)
 f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
   using F = Few<BM>;
   extern __shared__ uint8_t sm_raw[];
   // the same offset in every CTA of the cluster: their dynamic shared memory starts at the same address
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~(uintptr_t)1023);
-  float* part = reinterpret_cast<float*>(sm + (F::PART_BYTES ? F::STAGES * F::STAGE : 0));
-  float* scales = reinterpret_cast<float*>(sm + F::STAGES * F::STAGE + F::PART_BYTES);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + F::STAGES * F::STAGE + F::PART_BYTES + F::SCALE_BYTES);
+  float* part = reinterpret_cast<float*>(sm + F::STAGES * F::STAGE);
+  float* scales = reinterpret_cast<float*>(sm + F::STAGES * F::STAGE + F::PART);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + F::STAGES * F::STAGE + F::PART + F::SCALE_BYTES);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * F::STAGES + 2 * F::BUFS + 2);
   volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const uint32_t full = smem_u32(bars), stage_free = full + 8 * F::STAGES, acc_full = stage_free + 8 * F::STAGES, acc_free = acc_full + 8 * F::BUFS,
@@ -135,27 +206,16 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
   pdl_launch_dependents_small();  // behind the allocation: a dependent must not take columns that this grid still waits for
-  // the first meeting of the cluster: everybody's place for partial sums may be written
-  if (F::PART_BYTES && a.split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-
-  // The cluster meets twice before anybody's sums are complete (warps come from their roles): everybody's place for partial sums may be
-  // written, and everybody has sent, so that nobody leaves while something may still come
-  auto place_free = [&]() {
-    if (!F::PART_BYTES) {
-      __syncthreads();  // nobody here multiplies from the operands any more
-      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    }
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  };
+  // The cluster meets twice: everybody has started, so that partial sums may be sent, and (behind the sending) everybody has sent, so that
+  // nobody leaves while something may still come
+  if (a.split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 
   if (warp < F::EPI_WARPS) {
-    if (F::WIDE) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-    // ---- epilogue: warp w reads TMEM lanes 32 (w % 4) .. = weight rows, COLS of the activation rows
-    const int quad = warp & 3, col0 = (warp >> 2) * F::COLS;
-    constexpr int ET = F::EPI_WARPS * 32, MINE = F::AHEAD * BM / ET, CHUNK = F::COLS < 32 ? F::COLS : 32;
-    float2 acc[F::COLS / 2];
+    // ---- epilogue: warp w reads TMEM lanes 32 w .. = weight rows
+    constexpr int ET = F::EPI_WARPS * 32, MINE = F::AHEAD * BM / ET;
+    float2 acc[BM / 2];
 #pragma unroll
-    for (int i = 0; i < F::COLS / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+    for (int i = 0; i < BM / 2; ++i) acc[i] = make_float2(0.f, 0.f);
     float ahead[MINE];
     // scales of AHEAD blocks: thread t holds block t % AHEAD of activation rows t / AHEAD, ..
     auto fetch = [&](int first) {
@@ -188,65 +248,56 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t tl = tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(buf * BM + col0), freed = acc_free + 8 * buf;
-      const float4* sc = reinterpret_cast<const float4*>(half + at * F::SCALE_ROW + col0);
-      uint32_t v[2 * CHUNK / 16][16];
+      const uint32_t tl = tmem + ((uint32_t)(32 * warp) << 16) + (uint32_t)(buf * BM);
+      const float4* sc = reinterpret_cast<const float4*>(half + at * F::SCALE_ROW);
+      uint32_t v[BM / 16][16];
 #pragma unroll
-      for (int j = 0; j < CHUNK / 16; ++j) x_ld16(tl + 16 * j, v[j]);
+      for (int j = 0; j < BM / 16; ++j) x_ld16(tl + 16 * j, v[j]);
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      w_arrive(acc_free + 8 * buf);
 #pragma unroll
-      for (int c = 0; c < F::COLS / CHUNK; ++c) {
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (c + 1 < F::COLS / CHUNK) {
-#pragma unroll
-          for (int j = 0; j < CHUNK / 16; ++j) x_ld16(tl + CHUNK * (c + 1) + 16 * j, v[((c + 1) & 1) * (CHUNK / 16) + j]);
-        } else {
-          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-          __syncwarp();
-          w_arrive(freed);
-        }
-#pragma unroll
-        for (int j = 0; j < CHUNK / 4; ++j) {
-          const float4 f = sc[c * (CHUNK / 4) + j];
-          const uint32_t* p = &v[(c & 1) * (CHUNK / 16) + j / 4][4 * (j % 4)];
-          float2* to = acc + c * (CHUNK / 2) + 2 * j;
-          to[0] = fma2(make_float2(__uint_as_float(p[0]), __uint_as_float(p[1])), make_float2(f.x, f.y), to[0]);
-          to[1] = fma2(make_float2(__uint_as_float(p[2]), __uint_as_float(p[3])), make_float2(f.z, f.w), to[1]);
-        }
+      for (int j = 0; j < BM / 4; ++j) {
+        const float4 f = sc[j];
+        const uint32_t* p = &v[j / 4][4 * (j % 4)];
+        acc[2 * j] = fma2(make_float2(__uint_as_float(p[0]), __uint_as_float(p[1])), make_float2(f.x, f.y), acc[2 * j]);
+        acc[2 * j + 1] = fma2(make_float2(__uint_as_float(p[2]), __uint_as_float(p[3])), make_float2(f.z, f.w), acc[2 * j + 1]);
       }
       if (++buf == F::BUFS) { buf = 0; parity ^= 1u; }
     }
-    const int row = 32 * quad + lane, n = nt * 128 + row;
+    const int n = nt * 128 + tid;
     const float bias = a.out.bias && n < a.out.n ? a.out.bias[n] : 0.f;
     if (a.split == 1) {
       if (n < a.out.n)
 #pragma unroll
-        for (int j = 0; j < F::COLS; ++j)
-          if (m0 + col0 + j < a.out.m) f8_put(a.out, j & 1 ? acc[j / 2].y : acc[j / 2].x, bias, m0 + col0 + j, n);
+        for (int j = 0; j < BM; ++j)
+          if (m0 + j < a.out.m) f8_put(a.out, j & 1 ? acc[j / 2].y : acc[j / 2].x, bias, m0 + j, n);
     } else {
-      // the sums of the cluster's ranges of K: rank q gets activation rows BM q / split .. of all, [rank][weight row][activation row], and
-      // adds them in the order of the ranks
+      // The sums of the cluster's ranges of K: rank q gets activation rows BM q / split .. of all, [rank][weight row][activation row], and
+      // adds them in the order of the ranks. (Fetched by their owner between two meetings of the cluster they took 1.5 us longer.)
       const int per = BM / a.split;
-      const uint32_t mine = smem_u32(part) + (uint32_t)((rank * 128 + row) * per) * 4;
+      const uint32_t mine = smem_u32(part) + (uint32_t)((rank * 128 + tid) * per) * 4;
       __syncwarp();
-      place_free();
+      asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
       if (per >= 4) {
 #pragma unroll
-        for (int j = 0; j < F::COLS; j += 4) {
-          const int to = (col0 + j) / per;
-          st_cluster4(cluster_addr(mine + (uint32_t)(col0 + j - to * per) * 4, to), acc[j / 2], acc[j / 2 + 1], cluster_addr(joined, to));
+        for (int j = 0; j < BM; j += 4) {
+          const int to = j / per;
+          st_cluster4(cluster_addr(mine + (uint32_t)(j - to * per) * 4, to), acc[j / 2], acc[j / 2 + 1], cluster_addr(joined, to));
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < F::COLS; j += 2) st_cluster2(cluster_addr(mine, (col0 + j) / 2), acc[j / 2], cluster_addr(joined, (col0 + j) / 2));
+        for (int j = 0; j < BM; j += 2) st_cluster2(cluster_addr(mine, j / 2), acc[j / 2], cluster_addr(joined, j / 2));
       }
       __syncwarp();
       asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-      if (f_wait(joined, 0, dead, a.status)) {
-        for (int j = warp >> 2; j < per && m0 + rank * per + j < a.out.m; j += F::EPI_WARPS / 4) {
-          const float* from = part + row * per + j;
+      if (f_wait(joined, 0, dead, a.status) && n < a.out.n) {
+        for (int j = 0; j < per && m0 + rank * per + j < a.out.m; ++j) {
+          const float* from = part + tid * per + j;
           float v = 0.f;
           for (int q = 0; q < a.split; ++q) v += from[q * 128 * per];
-          if (n < a.out.n) f8_put(a.out, v, bias, m0 + rank * per + j, n);
+          f8_put(a.out, v, bias, m0 + rank * per + j, n);
         }
       }
       __syncwarp();
@@ -254,7 +305,6 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
       if (*dead) x_drain(joined, 0);
     }
   } else if (warp == F::EPI_WARPS) {
-    if (F::WIDE) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     // ---- copy requester, from the first activation rows on
     if (lane == 0) {
       pdl_wait();
@@ -272,34 +322,210 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
         for (int j = max(0, i - F::STAGES); j < i; ++j) x_drain(full + 8 * (j % F::STAGES), (uint32_t)((j / F::STAGES) & 1));
     }
   } else {
-    if (F::WIDE) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == F::EPI_WARPS + 1) {
-      // ---- MMA issuer
-      const uint64_t adesc0 = x_desc_rows(smem_u32(sm)), bdesc0 = x_desc_rows(smem_u32(sm) + F8_A_BYTES);
-      int st = 0, buf = 0;
-      uint32_t parity = 0, round = 0;
-      for (int i = 0; i < nkb; ++i) {
-        if (!f_wait(full + 8 * st, parity, dead, a.status)) break;
-        if (round && !f_wait(acc_free + 8 * buf, (round - 1) & 1, dead, a.status)) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint64_t at = (uint64_t)((st * F::STAGE) >> 4);
-        w_mma4_f8<2, 2>(tmem + (uint32_t)(buf * BM), adesc0 + at, bdesc0 + at, F::IDESC, 0u);
-        w_commit(acc_full + 8 * buf);
-        w_commit(stage_free + 8 * st);
-        if (++st == F::STAGES) { st = 0; parity ^= 1u; }
-        if (++buf == F::BUFS) { buf = 0; ++round; }
-      }
-      w_commit(drained);
-      x_drain(drained, 0);
+    // ---- MMA issuer
+    const uint64_t adesc0 = x_desc_rows(smem_u32(sm)), bdesc0 = x_desc_rows(smem_u32(sm) + F8_A_BYTES);
+    int st = 0, buf = 0;
+    uint32_t parity = 0, round = 0;
+    for (int i = 0; i < nkb; ++i) {
+      if (!f_wait(full + 8 * st, parity, dead, a.status)) break;
+      if (round && !f_wait(acc_free + 8 * buf, (round - 1) & 1, dead, a.status)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint64_t at = (uint64_t)((st * F::STAGE) >> 4);
+      w_mma4_f8<2, 2>(tmem + (uint32_t)(buf * BM), adesc0 + at, bdesc0 + at, F::IDESC, 0u);
+      w_commit(acc_full + 8 * buf);
+      w_commit(stage_free + 8 * st);
+      if (++st == F::STAGES) { st = 0; parity ^= 1u; }
+      if (++buf == F::BUFS) { buf = 0; ++round; }
     }
+    w_commit(drained);
+    x_drain(drained, 0);
   }
   if (warp >= F::EPI_WARPS && a.split > 1) {
     __syncwarp();
-    place_free();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
   __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(F::TMEM) : "memory");
+}
+
+// ---- some activation rows -----------------------------------------------------------------------------------------------
+
+// XR = 64 or 128 activation rows (in the M role, 128 lanes: lanes behind 64 rows multiply what lies behind them in shared memory and are not
+// read) by 128 weight rows per CTA
+template <int XR>
+struct Some {
+  static constexpr int EPI_WARPS = 8, THREADS = (EPI_WARPS + 3) * 32;
+  static constexpr int STAGE = XR * 128 + 128 * 128, STAGES = XR == 64 ? 8 : 6, BUFS = 4, TMEM = 512;
+  static constexpr int SMEM = STAGES * STAGE + 256 + 1024;
+  // instruction descriptor: f32 accumulator, e4m3 A and B, both K-major, N = 128, M = 128
+  static constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+  static_assert(STAGES % 2 == 0, "a stage belongs to one issuer");
+  static_assert(STAGES * STAGE >= XR * 512, "the sums take the operands' place");
+};
+
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int XR>
+__global__ void __launch_bounds__(Some<XR>::THREADS, 1)
+f8_some_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
+  using F = Some<XR>;
+  extern __shared__ uint8_t sm_raw[];
+  // the same offset in every CTA of the cluster: their dynamic shared memory starts at the same address
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + F::STAGES * F::STAGE);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * F::STAGES + 2 * F::BUFS + 1);
+  volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const uint32_t full = smem_u32(bars), stage_free = full + 8 * F::STAGES, acc_full = stage_free + 8 * F::STAGES, acc_free = acc_full + 8 * F::BUFS,
+                 drained = acc_free + 8 * F::BUFS;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = (int)cluster_rank(), tile = (int)blockIdx.x / a.split;
+  // activation tiles fastest: the CTAs that run together share their weight rows in L2
+  const int nt = tile / a.m_tiles, mt = tile - nt * a.m_tiles, m0 = mt * XR, n0 = nt * 128;
+  const int kb0 = (int)((long long)a.kblocks * rank / a.split), nkb = (int)((long long)a.kblocks * (rank + 1) / a.split) - kb0;
+  const int pre = min(F::STAGES, nkb);
+
+  if (tid == F::EPI_WARPS * 32) {  // as in f8_few_kernel
+    *dead = 0;
+    for (int i = 0; i < F::STAGES; ++i) { mbar_init(full + 8 * i, 1); mbar_init(stage_free + 8 * i, 1); }
+    for (int i = 0; i < F::BUFS; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_free + 8 * i, XR / 32 * 2); }
+    mbar_init(drained, 2);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    for (int i = 0; i < pre; ++i) {
+      mbar_expect_tx(full + 8 * i, F::STAGE);
+      x_tma_box2(smem_u32(sm + i * F::STAGE + XR * 128), &wmap, (kb0 + i) * F8_BLOCK, n0, full + 8 * i);
+    }
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(F::TMEM) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents_small();
+
+  const int quad = warp & 3, side = warp >> 2;
+  const bool reads = warp < F::EPI_WARPS && quad < XR / 32;
+  float2 acc[32];
+  if (reads) {
+    // ---- epilogue: warp w reads TMEM lanes 32 (w % 4) .. = activation rows, one half of the weight rows
+#pragma unroll
+    for (int i = 0; i < 32; ++i) acc[i] = make_float2(0.f, 0.f);
+    pdl_wait();
+    const float* sx = a.sx + (size_t)min(m0 + 32 * quad + lane, a.out.m - 1) * a.kblocks + kb0;
+    const float* sw = a.sw + (size_t)nt * a.kblocks + kb0;
+    float fx = nkb ? sx[0] : 0.f, fw = nkb ? sw[0] : 0.f;
+    int buf = 0;
+    uint32_t parity = 0;
+#pragma unroll 1
+    for (int i = 0; i < nkb; ++i) {
+      if (!f_wait(acc_full + 8 * buf, parity, dead, a.status)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t tl = tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(buf * 128 + side * 64);
+      uint32_t v[4][16];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x_ld16(tl + 16 * j, v[j]);
+      const float2 f = make_float2(fx * fw, fx * fw);
+      fx = sx[min(i + 1, nkb - 1)];  // in flight until the next block
+      fw = sw[min(i + 1, nkb - 1)];
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      w_arrive(acc_free + 8 * buf);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) acc[j] = fma2(make_float2(__uint_as_float(v[j / 8][2 * j % 16]), __uint_as_float(v[j / 8][2 * j % 16 + 1])), f, acc[j]);
+      if (++buf == F::BUFS) { buf = 0; parity ^= 1u; }
+    }
+  } else if (warp == F::EPI_WARPS) {
+    // ---- copy requester, from the first activation rows on
+    if (lane == 0) {
+      pdl_wait();
+      int i = 0;
+      for (; i < pre; ++i) x_tma_box2(smem_u32(sm + i * F::STAGE), &xmap, (kb0 + i) * F8_BLOCK, m0, full + 8 * i);
+      for (; i < nkb; ++i) {
+        const int s = i % F::STAGES;
+        if (!x_wait(stage_free + 8 * s, (uint32_t)((i / F::STAGES - 1) & 1), dead, a.status)) break;
+        const uint32_t dst = smem_u32(sm + s * F::STAGE), bar = full + 8 * s;
+        mbar_expect_tx(bar, F::STAGE);
+        x_tma_box2(dst + XR * 128, &wmap, (kb0 + i) * F8_BLOCK, n0, bar);
+        x_tma_box2(dst, &xmap, (kb0 + i) * F8_BLOCK, m0, bar);
+      }
+      if (*dead)
+        for (int j = max(0, i - F::STAGES); j < i; ++j) x_drain(full + 8 * (j % F::STAGES), (uint32_t)((j / F::STAGES) & 1));
+    }
+  } else if (warp > F::EPI_WARPS) {
+    // ---- two MMA issuers, every other block each
+    const uint64_t adesc0 = x_desc_rows(smem_u32(sm)), bdesc0 = x_desc_rows(smem_u32(sm) + XR * 128);
+    const int which = warp - F::EPI_WARPS - 1;
+    int st = which;
+    uint32_t parity = 0;
+    for (int i = which; i < nkb; i += 2) {
+      const int buf = i % F::BUFS;
+      if (!f_wait(full + 8 * st, parity, dead, a.status)) break;
+      if (i >= F::BUFS && !f_wait(acc_free + 8 * buf, (uint32_t)(i / F::BUFS - 1) & 1u, dead, a.status)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint64_t at = (uint64_t)((st * F::STAGE) >> 4);
+      w_mma4_f8<2, 2>(tmem + (uint32_t)(buf * 128), adesc0 + at, bdesc0 + at, F::IDESC, 0u);
+      w_commit(acc_full + 8 * buf);
+      w_commit(stage_free + 8 * st);
+      if ((st += 2) >= F::STAGES) { st -= F::STAGES; parity ^= 1u; }
+    }
+    w_commit(drained);
+    x_drain(drained, 0);
+  }
+  __syncthreads();  // nobody here multiplies from the operands any more: they make room for the sums
+  pdl_wait();       // for the warps that have not been in a role that waits
+
+  if (a.split == 1) {
+    if (reads) f8_store_rows<64>(a.out, acc, sm + warp * TURN_BYTES, m0 + 32 * quad, n0 + 64 * side);
+  } else {
+    // The sums of the cluster's ranges of K: everybody lays down its own, 512 bytes a row, 16-byte piece p of row r at place p ^ (r % 8);
+    // rank q fetches rows XR q / split .. of all and adds them in the order of the ranks, a warp to a row.
+    if (reads) {
+      const int r = 32 * quad + lane;
+#pragma unroll
+      for (int p = 0; p < 16; ++p)
+        *reinterpret_cast<float4*>(sm + r * 512 + (((16 * side + p) ^ (r & 7)) << 4)) = make_float4(acc[2 * p].x, acc[2 * p].y, acc[2 * p + 1].x, acc[2 * p + 1].y);
+    }
+    __syncwarp();
+    cluster_sync();
+    const int per = XR / a.split, end = min((rank + 1) * per, a.out.m - m0);
+    if (warp < F::EPI_WARPS) {
+#pragma unroll 2
+      for (int r = rank * per + warp; r < end; r += F::EPI_WARPS) {
+        const uint32_t from = smem_u32(sm + r * 512 + ((lane ^ (r & 7)) << 4));
+        float4 v = ld_cluster4(cluster_addr(from, 0));
+#pragma unroll
+        for (int q = 1; q < 8; ++q)
+          if (q < a.split) {
+            const float4 u = ld_cluster4(cluster_addr(from, (uint32_t)q));
+            v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+          }
+        const int n = n0 + 4 * lane;
+        const float* b = a.out.bias;
+        if (a.out.vec) {
+          if (n < a.out.n) f8_put4(a.out, v, b ? make_float4(b[n], b[n + 1], b[n + 2], b[n + 3]) : make_float4(0.f, 0.f, 0.f, 0.f), m0 + r, n);
+        } else {
+          const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (n + i < a.out.n) f8_put(a.out, e[i], b ? b[n + i] : 0.f, m0 + r, n + i);
+        }
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // the others may still read
+  }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(F::TMEM) : "memory");
@@ -310,8 +536,6 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
 // Two warpgroups of epilogue warps and one of the copy requester and the issuer, which hands its registers over: 384 x 168 at launch are
 // 256 x 224 + 128 x 56. A thread holds 128 sums and 64 values on their way.
 constexpr int PAIR_EPI_WARPS = 8, PAIR_THREADS = (PAIR_EPI_WARPS + 4) * 32, PAIR_MAX_STAGES = 8;
-constexpr int TURN_BYTES = 32 * 128;  // a warp's 32 rows x 128 bytes on their way out, 16-byte piece p of row r at place p ^ (r % 8)
-
 template <int NW>
 struct Pair {
   static constexpr int STAGE = F8_A_BYTES + NW / 2 * 128, STAGES = NW == 256 ? 6 : 8, TMEM = 512;
@@ -325,83 +549,8 @@ struct PairArgs {
   const float *sx, *sw;
   F8Out out;
   int kblocks, m_tiles, n_tiles, m_group;
-  int vec;   // four columns of y (and of the residuals) are aligned
-  int pack;  // 16-bit y without residual or bias, eight columns aligned: rounded before they are turned
   int* status;
 };
-
-__device__ __forceinline__ uint32_t f8_pair(const F8Out& o, float2 v) {
-  const __nv_bfloat162 b = __floats2bfloat162_rn(v.x, v.y);
-  const __half2 h = __floats2half2_rn(v.x, v.y);
-  return o.type == FB200_BF16 ? *reinterpret_cast<const uint32_t*>(&b) : *reinterpret_cast<const uint32_t*>(&h);
-}
-// Four neighbouring outputs
-__device__ __forceinline__ void f8_put4(const F8Out& o, float4 v, const float4& bias, int m, int n) {
-  const size_t at = (size_t)m * o.n + n;
-  v.x += bias.x; v.y += bias.y; v.z += bias.z; v.w += bias.w;
-  if (o.r1) { const float4 r = *reinterpret_cast<const float4*>(o.r1 + at); v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w; }
-  if (o.r2) { const float4 r = *reinterpret_cast<const float4*>(o.r2 + at); v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w; }
-  if (o.type == FB200_F32) {
-    *reinterpret_cast<float4*>(reinterpret_cast<float*>(o.y) + at) = v;
-  } else {
-    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(o.y) + at) = make_uint2(f8_pair(o, make_float2(v.x, v.y)), f8_pair(o, make_float2(v.z, v.w)));
-  }
-}
-
-// A warp's 32 rows from m0 on, COLS columns from n0 on, a row per thread, to y: turned in shared memory, so that a row's columns leave
-// together.
-template <int COLS>
-__device__ __forceinline__ void f8_store_rows(const PairArgs& a, const float2 (&acc)[COLS / 2], uint8_t* turn, int m0, int n0) {
-  const int lane = threadIdx.x & 31, m_end = a.out.m - m0, n_end = a.out.n - n0;
-  if (a.pack) {
-    const uint8_t* from = turn + (lane >> 3) * 128;
-    uint16_t* to = reinterpret_cast<uint16_t*>(a.out.y) + (size_t)m0 * a.out.n + n0 + 8 * (lane & 7);
-#pragma unroll
-    for (int c = 0; c < COLS / 64; ++c) {
-      if (64 * c >= n_end) break;
-      __syncwarp();
-#pragma unroll
-      for (int p = 0; p < 8; ++p) {
-        const float2* v = acc + 32 * c + 4 * p;
-        *reinterpret_cast<uint4*>(turn + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_uint4(f8_pair(a.out, v[0]), f8_pair(a.out, v[1]), f8_pair(a.out, v[2]), f8_pair(a.out, v[3]));
-      }
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = 4 * i + (lane >> 3);
-        const uint4 v = *reinterpret_cast<const uint4*>(from + 512 * i + (((lane & 7) ^ (r & 7)) << 4));
-        if (r < m_end && 64 * c + 8 * (lane & 7) < n_end) *reinterpret_cast<uint4*>(to + (size_t)r * a.out.n + 64 * c) = v;
-      }
-    }
-    return;
-  }
-#pragma unroll
-  for (int c = 0; c < COLS / 32; ++c) {
-    if (32 * c >= n_end) break;
-    __syncwarp();
-#pragma unroll
-    for (int p = 0; p < 8; ++p) {
-      const float2* v = acc + 16 * c + 2 * p;
-      *reinterpret_cast<float4*>(turn + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
-    }
-    __syncwarp();
-    if (a.vec) {  // whole fours: N is a multiple of four then
-      const int n = n0 + 32 * c + 4 * (lane & 7);
-      if (n >= a.out.n) continue;
-      const float4 bias = a.out.bias ? make_float4(a.out.bias[n], a.out.bias[n + 1], a.out.bias[n + 2], a.out.bias[n + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int r = lane >> 3; r < min(32, m_end); r += 4)
-        f8_put4(a.out, *reinterpret_cast<const float4*>(turn + r * 128 + (((lane & 7) ^ (r & 7)) << 4)), bias, m0 + r, n);
-    } else {
-      const int n = n0 + 32 * c + lane;
-      if (n >= a.out.n) continue;
-      const float bias = a.out.bias ? a.out.bias[n] : 0.f;
-#pragma unroll 8
-      for (int r = 0; r < min(32, m_end); ++r)
-        f8_put(a.out, *reinterpret_cast<const float*>(turn + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3)), bias, m0 + r, n);
-    }
-  }
-}
 
 template <int NW>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
@@ -504,7 +653,7 @@ f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const
       if (!alive) break;
       const int m_done = m_first, n_done = n_first;
       if (item + npairs < items) begin(item + npairs);  // its first scales arrive meanwhile
-      f8_store_rows<HALF>(a, acc, turn + warp * TURN_BYTES, m_done, n_done);
+      f8_store_rows<HALF>(a.out, acc, turn + warp * TURN_BYTES, m_done, n_done);
     }
   } else if (warp == PAIR_EPI_WARPS) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -588,22 +737,21 @@ int allow_smem(fb200_device* dev, K kern, int bytes, bool (&configured)[64]) {
   return FB200_OK;
 }
 
-template <int BM>
-int launch_few(fb200_device* dev, const F8Job& j, int split) {
-  using F = Few<BM>;
-  static bool configured[64] = {false};
-  int rc = allow_smem(dev, f8_few_kernel<BM>, F::SMEM, configured);
+// The kernels of single CTAs: clusters of `split` CTAs per tile of `rows` activation rows and 128 weight rows
+template <typename K>
+int launch_split(fb200_device* dev, const F8Job& j, K kern, int rows, int threads, int smem, int split, bool (&configured)[64]) {
+  int rc = allow_smem(dev, kern, smem, configured);
   if (rc) return rc;
   CUtensorMap xmap;
-  if (!fb200_make_map_2d_bytes(&xmap, j.x, j.w->k, (uint64_t)j.out.m, j.ld, BM))
+  if (!fb200_make_map_2d_bytes(&xmap, j.x, j.w->k, (uint64_t)j.out.m, j.ld, (uint32_t)rows))
     return fb200_fail(dev, FB200_ERR_CUDA, "f8_mat_mul: tensor map refused (x %d rows every %zu bytes)", j.out.m, j.ld);
-  const FewArgs a = {j.sx, j.w->scales, j.out, j.kblocks, (j.out.m + BM - 1) / BM, split, dev->status};
+  const FewArgs a = {j.sx, j.w->scales, j.out, j.kblocks, (j.out.m + rows - 1) / rows, split, dev->status};
   const long long ctas = (long long)a.m_tiles * ((j.out.n + 127) / 128) * split;
   if (ctas > 0x7FFFFFFF) return fb200_fail(dev, FB200_ERR_INVALID_SHAPE, "f8_mat_mul: %d x %d outputs are too many", j.out.m, j.out.n);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(F::THREADS);
-  cfg.dynamicSmemBytes = F::SMEM;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = dev->stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -613,9 +761,19 @@ int launch_few(fb200_device* dev, const F8Job& j, int split) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = dev->pdl ? 2 : 1;
-  FB_CUDA(dev, cudaLaunchKernelEx(&cfg, f8_few_kernel<BM>, a, j.w->map128, xmap));
+  FB_CUDA(dev, cudaLaunchKernelEx(&cfg, kern, a, j.w->map128, xmap));
   dev->launches++;
   return FB200_OK;
+}
+template <int BM>
+int launch_few(fb200_device* dev, const F8Job& j, int split) {
+  static bool configured[64] = {false};
+  return launch_split(dev, j, f8_few_kernel<BM>, BM, Few<BM>::THREADS, Few<BM>::SMEM, split, configured);
+}
+template <int XR>
+int launch_some(fb200_device* dev, const F8Job& j, int split) {
+  static bool configured[64] = {false};
+  return launch_split(dev, j, f8_some_kernel<XR>, XR, Some<XR>::THREADS, Some<XR>::SMEM, split, configured);
 }
 
 template <int NW>
@@ -627,15 +785,12 @@ int launch_pair(fb200_device* dev, const F8Job& j) {
   CUtensorMap xmap;
   if (!fb200_make_map_2d_bytes(&xmap, j.x, j.w->k, (uint64_t)j.out.m, j.ld, 128))
     return fb200_fail(dev, FB200_ERR_CUDA, "f8_mat_mul: tensor map refused (x %d rows every %zu bytes)", j.out.m, j.ld);
-  PairArgs a = {j.sx, j.w->scales, j.out, j.kblocks, (j.out.m + 255) / 256, (j.out.n + NW - 1) / NW, 1, 0, 0, dev->status};
+  PairArgs a = {j.sx, j.w->scales, j.out, j.kblocks, (j.out.m + 255) / 256, (j.out.n + NW - 1) / NW, 1, dev->status};
   const long long items = (long long)a.m_tiles * a.n_tiles;
   if (items > 0x3FFFFFFF) return fb200_fail(dev, FB200_ERR_INVALID_SHAPE, "f8_mat_mul: %d x %d outputs are too many", j.out.m, j.out.n);
   // the activation rows of a group take at most 32 MB of L2
   const long long fit = (32ll << 20) / (256ll * F8_BLOCK * j.kblocks);
   a.m_group = fit < 1 ? 1 : fit > a.m_tiles ? a.m_tiles : (int)fit;
-  const uintptr_t four = j.out.type == FB200_F32 ? 16 : 8;
-  a.pack = j.out.type != FB200_F32 && !j.out.bias && !j.out.r1 && !j.out.r2 && j.out.n % 8 == 0 && (uintptr_t)j.out.y % 16 == 0;
-  a.vec = j.out.n % 4 == 0 && (uintptr_t)j.out.y % four == 0 && (uintptr_t)j.out.r1 % 16 == 0 && (uintptr_t)j.out.r2 % 16 == 0;
   const int pairs = items < dev->sm_count / 2 ? (int)items : dev->sm_count / 2;
   return fb200_launch(dev, f8_pair_kernel<NW>, dim3((unsigned)(2 * pairs)), dim3(PAIR_THREADS), (size_t)P::SMEM, true, a,
                       j.w->map64, xmap);
@@ -643,28 +798,27 @@ int launch_pair(fb200_device* dev, const F8Job& j) {
 
 int f8_product(fb200_device* dev, const F8Job& j) {
   const int m = j.out.m, n_tiles = (j.out.n + 127) / 128;
-  int bm = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256, split = 1, pair = 0;
-  const int tiles = n_tiles * ((m + bm - 1) / bm);
-  while (split < 8 && tiles * split * 2 <= dev->sm_count * (bm <= 64 ? 2 : 1) && j.kblocks >= split * 4) split *= 2;
+  int rows = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128, split = 1, pair = 0;
+  const int tiles = n_tiles * ((m + rows - 1) / rows);
+  while (split < 8 && tiles * split * 2 <= dev->sm_count * (rows <= 32 ? 2 : 1) && j.kblocks >= split * 4) split *= 2;
   if (m > 256) pair = 256;
-  // FB200_F8_TILE (tests, tuning; read per call): "BM,SPLIT" activation rows and ranges of K of the kernel for few rows, "pair,NW" pairs
-  // with 128 or 256 weight rows; what there is not leaves the choice to the rule
+  // FB200_F8_TILE (tests, tuning; read per call): "ROWS,SPLIT" activation rows (16, 32, 64, 128) and ranges of K of the kernels on single
+  // CTAs, "pair,NW" pairs with 128 or 256 weight rows; what there is not leaves the choice to the rule
   if (const char* cfg = getenv("FB200_F8_TILE")) {
-    int fbm, fsplit;
-    if (sscanf(cfg, "pair,%d", &fbm) == 1) {
-      if (fbm == 128 || fbm == 256) pair = fbm;
-    } else if (sscanf(cfg, "%d,%d", &fbm, &fsplit) == 2 && (fbm == 16 || fbm == 32 || fbm == 64 || fbm == 128 || fbm == 256) &&
+    int frows, fsplit;
+    if (sscanf(cfg, "pair,%d", &frows) == 1) {
+      if (frows == 128 || frows == 256) pair = frows;
+    } else if (sscanf(cfg, "%d,%d", &frows, &fsplit) == 2 && (frows == 16 || frows == 32 || frows == 64 || frows == 128) &&
                (fsplit == 1 || fsplit == 2 || fsplit == 4 || fsplit == 8)) {
-      bm = fbm, split = fsplit, pair = 0;
+      rows = frows, split = fsplit, pair = 0;
     }
   }
   if (pair) return pair == 128 ? launch_pair<128>(dev, j) : launch_pair<256>(dev, j);
-  switch (bm) {
+  switch (rows) {
     case 16: return launch_few<16>(dev, j, split);
     case 32: return launch_few<32>(dev, j, split);
-    case 64: return launch_few<64>(dev, j, split);
-    case 128: return launch_few<128>(dev, j, split);
-    default: return launch_few<256>(dev, j, split);
+    case 64: return launch_some<64>(dev, j, split);
+    default: return launch_some<128>(dev, j, split);
   }
 }
 
@@ -784,9 +938,12 @@ int fb200_f8_mat_mul(fb200_device* dev, const uint8_t* codes_dev, size_t ld, con
   if (epi != FB200_EPI_NONE && ((uintptr_t)ep->r1_dev % 4 || (uintptr_t)ep->r2_dev % 4))
     return fb200_fail(dev, FB200_ERR_INVALID_ARGUMENT, "f8_mat_mul: r1 or r2 is not aligned");
   if (m == 0) return FB200_OK;
-  F8Job j = {codes_dev, ld, scales_dev, w, {y_dev, y_type, nullptr, nullptr, nullptr, (int)m, (int)w->n}, (int)((w->k + 127) / 128)};
+  F8Job j = {codes_dev, ld, scales_dev, w, {y_dev, y_type, nullptr, nullptr, nullptr, (int)m, (int)w->n, 0, 0}, (int)((w->k + 127) / 128)};
   if (epi == FB200_EPI_BIAS) j.out.bias = ep->r1_dev;
   if (epi == FB200_EPI_RESIDUAL) { j.out.r1 = ep->r1_dev; j.out.r2 = ep->r2_dev; }
+  const uintptr_t four = y_type == FB200_F32 ? 16 : 8;
+  j.out.vec = w->n % 4 == 0 && (uintptr_t)y_dev % four == 0 && (uintptr_t)j.out.r1 % 16 == 0 && (uintptr_t)j.out.r2 % 16 == 0;
+  j.out.pack = y_type != FB200_F32 && epi == FB200_EPI_NONE && w->n % 8 == 0 && (uintptr_t)y_dev % 16 == 0;
   fb200_op_trace scope(dev, m <= 32 ? "f8_mat_mul (1..32 rows)" : "f8_mat_mul (> 32 rows)",
                        (double)w->n * (double)w->k + (double)m * ((double)w->k + (y_type == FB200_F32 ? 4.0 : 2.0) * (double)w->n));
   return f8_product(dev, j);

@@ -205,7 +205,7 @@ def test_rms_norm_of_zero_and_not_finite_rows(dev):
 
 # ---- the product --------------------------------------------------------------------------------------------------------
 
-TILES = ["16,1", "16,2", "16,4", "16,8", "32,1", "32,4", "64,1", "64,2", "64,8", "128,1", "128,2", "128,4", "256,1", "256,2", "256,8", "pair,128", "pair,256"]
+TILES = ["16,1", "16,2", "16,4", "16,8", "32,1", "32,4", "32,8", "64,1", "64,2", "64,8", "128,1", "128,2", "128,4", "128,8", "pair,128", "pair,256"]
 
 
 def operands(rng, m, n, k):
@@ -269,7 +269,7 @@ def test_product_rows(dev, m, n, k):
 
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("epilogue,second", [(kb.EPI_NONE, False), (kb.EPI_RESIDUAL, False), (kb.EPI_RESIDUAL, True), (kb.EPI_BIAS, False)])
-@pytest.mark.parametrize("tile,m", [("16,2", 5), ("128,1", 100), ("256,4", 300), ("pair,128", 300), ("pair,256", 300)])
+@pytest.mark.parametrize("tile,m", [("16,2", 5), ("64,1", 60), ("128,4", 300), ("pair,128", 300), ("pair,256", 300)])
 @pytest.mark.parametrize("n", [260, 333])
 def test_product_epilogues(dev, monkeypatch, kind, epilogue, second, tile, m, n):
     monkeypatch.setenv("FB200_F8_TILE", tile)
@@ -281,7 +281,7 @@ def test_product_model_sizes(dev, m, n, k):
     run_product(dev, np.random.default_rng(k), m, n, k, "bf16", kb.EPI_RESIDUAL)
 
 
-@pytest.mark.parametrize("tile,m", [("16,4", 9), ("64,2", 50), ("128,1", 100), ("256,2", 260), ("pair,128", 260), ("pair,256", 260)])
+@pytest.mark.parametrize("tile,m", [("16,4", 9), ("64,2", 50), ("128,2", 260), ("pair,128", 260), ("pair,256", 260)])
 def test_product_is_repeatable(dev, monkeypatch, tile, m):
     monkeypatch.setenv("FB200_F8_TILE", tile)
     x, xs, w, ws = operands(np.random.default_rng(m), m, 1300, 2000)
@@ -291,7 +291,7 @@ def test_product_is_repeatable(dev, monkeypatch, tile, m):
         assert np.array_equal(rows.f8_mat_mul(mat).as_slice(), first)
 
 
-@pytest.mark.parametrize("tile,m", [("16,2", 9), ("128,1", 100), ("256,2", 260), ("pair,128", 260), ("pair,256", 260)])
+@pytest.mark.parametrize("tile,m", [("16,2", 9), ("128,2", 260), ("pair,128", 260), ("pair,256", 260)])
 def test_product_keeps_what_is_not_finite_in_its_row_and_column(dev, monkeypatch, tile, m):
     monkeypatch.setenv("FB200_F8_TILE", tile)
     x, xs, w, ws = operands(np.random.default_rng(m), m, 400, 600)
