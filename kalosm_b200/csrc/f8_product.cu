@@ -74,13 +74,31 @@ __device__ __forceinline__ void f8_put4(const F8Out& o, float4 v, const float4& 
   }
 }
 
+// Turned rows of 32 f32 columns to y, `rows` of them from m0 on; the lane's column is on the matrix
+__device__ __forceinline__ void f8_rows_out(const F8Out& o, const uint8_t* turn, int rows, int m0, int n) {
+  const float bias = o.bias ? o.bias[n] : 0.f;
+  const uintptr_t from = reinterpret_cast<uintptr_t>(turn) + 4 * (threadIdx.x & 31);
+  const size_t first = (size_t)m0 * o.n + n;
+  const int size = o.type == FB200_F32 ? 4 : 2;
+  uint8_t* to = reinterpret_cast<uint8_t*>(o.y) + first * size;
+  const float *p1 = o.r1 + first, *p2 = o.r2 + first;
+#pragma unroll 8
+  for (int r = 0; r < rows; ++r, to += (size_t)o.n * size) {
+    float v = *reinterpret_cast<const float*>((from ^ ((r & 7) << 4)) + r * 128) + bias;
+    if (o.r1) v += p1[(size_t)r * o.n];
+    if (o.r2) v += p2[(size_t)r * o.n];
+    if (size == 4) *reinterpret_cast<float*>(to) = v;
+    else *reinterpret_cast<uint16_t*>(to) = (uint16_t)f8_pair(o, make_float2(v, 0.f));
+  }
+}
+
 // A warp's 32 rows from m0 on, COLS columns from n0 on, a row per thread, to y: turned in shared memory, so that a row's columns leave
 // together.
 template <int COLS>
 __device__ __forceinline__ void f8_store_rows(const F8Out& o, const float2 (&acc)[COLS / 2], uint8_t* turn, int m0, int n0) {
-  const int lane = threadIdx.x & 31, m_end = o.m - m0, n_end = o.n - n0;
+  const int lane = threadIdx.x & 31, rows = min(32, o.m - m0), n_end = o.n - n0;
+  uint4* mine = reinterpret_cast<uint4*>(turn + lane * 128);
   if (o.pack) {
-    const uint8_t* from = turn + (lane >> 3) * 128;
     uint16_t* to = reinterpret_cast<uint16_t*>(o.y) + (size_t)m0 * o.n + n0 + 8 * (lane & 7);
 #pragma unroll
     for (int c = 0; c < COLS / 64; ++c) {
@@ -89,14 +107,14 @@ __device__ __forceinline__ void f8_store_rows(const F8Out& o, const float2 (&acc
 #pragma unroll
       for (int p = 0; p < 8; ++p) {
         const float2* v = acc + 32 * c + 4 * p;
-        *reinterpret_cast<uint4*>(turn + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_uint4(f8_pair(o, v[0]), f8_pair(o, v[1]), f8_pair(o, v[2]), f8_pair(o, v[3]));
+        mine[p ^ (lane & 7)] = make_uint4(f8_pair(o, v[0]), f8_pair(o, v[1]), f8_pair(o, v[2]), f8_pair(o, v[3]));
       }
       __syncwarp();
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int r = 4 * i + (lane >> 3);
-        const uint4 v = *reinterpret_cast<const uint4*>(from + 512 * i + (((lane & 7) ^ (r & 7)) << 4));
-        if (r < m_end && 64 * c + 8 * (lane & 7) < n_end) *reinterpret_cast<uint4*>(to + (size_t)r * o.n + 64 * c) = v;
+        const uint4 v = *reinterpret_cast<const uint4*>(turn + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+        if (r < rows && 64 * c + 8 * (lane & 7) < n_end) *reinterpret_cast<uint4*>(to + (size_t)r * o.n + 64 * c) = v;
       }
     }
     return;
@@ -108,23 +126,19 @@ __device__ __forceinline__ void f8_store_rows(const F8Out& o, const float2 (&acc
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
       const float2* v = acc + 16 * c + 2 * p;
-      *reinterpret_cast<float4*>(turn + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+      mine[p ^ (lane & 7)] = make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
     }
     __syncwarp();
     if (o.vec) {  // whole fours: N is a multiple of four then
       const int n = n0 + 32 * c + 4 * (lane & 7);
-      if (n >= o.n) continue;
-      const float4 bias = o.bias ? make_float4(o.bias[n], o.bias[n + 1], o.bias[n + 2], o.bias[n + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+      if (n < o.n) {
+        const float4 bias = o.bias ? make_float4(o.bias[n], o.bias[n + 1], o.bias[n + 2], o.bias[n + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-      for (int r = lane >> 3; r < min(32, m_end); r += 4)
-        f8_put4(o, *reinterpret_cast<const float4*>(turn + r * 128 + (((lane & 7) ^ (r & 7)) << 4)), bias, m0 + r, n);
-    } else {
-      const int n = n0 + 32 * c + lane;
-      if (n >= o.n) continue;
-      const float bias = o.bias ? o.bias[n] : 0.f;
-#pragma unroll 8
-      for (int r = 0; r < min(32, m_end); ++r)
-        f8_put(o, *reinterpret_cast<const float*>(turn + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3)), bias, m0 + r, n);
+        for (int r = lane >> 3; r < rows; r += 4)
+          f8_put4(o, *reinterpret_cast<const float4*>(turn + r * 128 + (((lane & 7) ^ (r & 7)) << 4)), bias, m0 + r, n);
+      }
+    } else if (32 * c + lane < n_end) {
+      f8_rows_out(o, turn, rows, m0, n0 + 32 * c + lane);
     }
   }
 }
@@ -569,19 +583,20 @@ f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const
                  acc_free = acc_full + 32, drained = acc_free + 32;
   const int items = a.m_tiles * a.n_tiles;
 
-  if (tid == 0) {
+  // The copy requester sets the barriers up and asks for the first weights, which depend on no kernel in front, as soon as both CTAs' are
+  // there; tensor memory is allocated meanwhile
+  if (tid == PAIR_EPI_WARPS * 32) {
     *dead = 0;
     for (int i = 0; i < P::STAGES; ++i) { mbar_init(full + 8 * i, 1); mbar_init(stage_free + 8 * i, P::PARTS); }
     for (int i = 0; i < 4; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_free + 8 * i, 2 * PAIR_EPI_WARPS / P::PARTS); }
     mbar_init(drained, 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   if (warp == 0) pair_tmem_alloc(smem_u32(tmem_slot), P::TMEM);
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
-  cluster_sync();
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = *tmem_slot;
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 
   // Tiles in groups of m_group activation tiles, activation tiles fastest within a group: the pairs that run together share their
   // weight rows in L2, and a group's activation rows stay there while the weights go by.
@@ -591,6 +606,26 @@ f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const
     nt = at / height;
     mt = first + at - nt * height;
   };
+  const int pre = min(P::STAGES, a.kblocks);
+  // of every 128 columns of a product a CTA holds 64 weight rows
+  auto weights = [&](int s, int kb, int nt) {
+#pragma unroll
+    for (int p = 0; p < P::PARTS; ++p)
+      pair_tma_box2(smem_u32(sm + s * P::STAGE) + F8_A_BYTES + p * 64 * 128, &wmap, kb * F8_BLOCK, nt * NW + 128 * p + rank * 64, cluster_addr(full + 8 * s, 0));
+  };
+  if (tid == PAIR_EPI_WARPS * 32) {
+    int mt, nt;
+    split(pair, mt, nt);
+    for (int s = 0; s < pre; ++s) {
+      if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * P::STAGE);
+      weights(s, s, nt);
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents_small();  // behind the allocation: a dependent must not take columns that this grid still waits for
 
   if (warp < PAIR_EPI_WARPS) {
     // ---- epilogue: warp w reads TMEM lanes 32 (w % 4) .. of this CTA's 128 activation rows, one half of the weight rows
@@ -666,15 +701,14 @@ f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const
       for (int item = pair; item < items && alive; item += npairs) {
         int mt, nt;
         split(item, mt, nt);
-        const int xr = mt * 256 + rank * 128, wr = nt * NW + rank * 64;  // of every 128 columns of a product a CTA holds 64 weight rows
         for (int kb = 0; kb < a.kblocks; ++kb, ++k) {
           const int s = k % P::STAGES, round = k / P::STAGES;
           if (round > 0 && !(alive = x_wait(stage_free + 8 * s, (uint32_t)((round - 1) & 1), dead, a.status))) break;
-          const uint32_t dst = smem_u32(sm + s * P::STAGE), bar = cluster_addr(full + 8 * s, 0);
-          if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * P::STAGE);
-          pair_tma_box2(dst, &xmap, kb * F8_BLOCK, xr, bar);
-#pragma unroll
-          for (int p = 0; p < P::PARTS; ++p) pair_tma_box2(dst + F8_A_BYTES + p * 64 * 128, &wmap, kb * F8_BLOCK, wr + 128 * p, bar);
+          if (k >= pre) {
+            if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * P::STAGE);
+            weights(s, kb, nt);
+          }
+          pair_tma_box2(smem_u32(sm + s * P::STAGE), &xmap, kb * F8_BLOCK, mt * 256 + rank * 128, cluster_addr(full + 8 * s, 0));
         }
       }
       if (*dead) {
