@@ -387,6 +387,52 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
   return v;
 }
 
+// Rows XR rank / SPLIT .. of the sums that the CTAs of the cluster have laid down, added in the order of the ranks, a warp to a row at a
+// time; all loads of a warp are in flight together. Tells the cluster when it has read.
+template <int XR, int SPLIT>
+__device__ __forceinline__ void f8_join(const F8Out& o, const uint8_t* sm, int rank, int warp, int m0, int n0) {
+  constexpr int PER = XR / SPLIT, ROWS = PER / 8;
+  const int lane = threadIdx.x & 31, first = rank * PER + warp;
+  float4 v[ROWS][SPLIT];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = first + 8 * i;
+    const uint32_t from = smem_u32(sm + r * 512 + ((lane ^ (r & 7)) << 4));
+    if (m0 + r < o.m)
+#pragma unroll
+      for (int q = 0; q < SPLIT; ++q) v[i][q] = ld_cluster4(cluster_addr(from, (uint32_t)q));
+  }
+  const int n = n0 + 4 * lane;
+  float4 bias = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (o.bias) {
+    if (n < o.n) bias.x = o.bias[n];
+    if (n + 1 < o.n) bias.y = o.bias[n + 1];
+    if (n + 2 < o.n) bias.z = o.bias[n + 2];
+    if (n + 3 < o.n) bias.w = o.bias[n + 3];
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+    for (int q = 1; q < SPLIT; ++q) {
+      v[i][0].x += v[i][q].x; v[i][0].y += v[i][q].y; v[i][0].z += v[i][q].z; v[i][0].w += v[i][q].w;
+    }
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int m = m0 + first + 8 * i;
+    if (m >= o.m) break;
+    if (o.vec) {
+      if (n < o.n) f8_put4(o, v[i][0], bias, m, n);
+    } else {
+      const float e[4] = {v[i][0].x, v[i][0].y, v[i][0].z, v[i][0].w}, b[4] = {bias.x, bias.y, bias.z, bias.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n + j < o.n) f8_put(o, e[j], b[j], m, n + j);
+    }
+  }
+}
+
 template <int XR>
 __global__ void __launch_bounds__(Some<XR>::THREADS, 1)
 f8_some_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
@@ -513,32 +559,15 @@ f8_some_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const 
     }
     __syncwarp();
     cluster_sync();
-    const int per = XR / a.split, end = min((rank + 1) * per, a.out.m - m0);
     if (warp < F::EPI_WARPS) {
-#pragma unroll 2
-      for (int r = rank * per + warp; r < end; r += F::EPI_WARPS) {
-        const uint32_t from = smem_u32(sm + r * 512 + ((lane ^ (r & 7)) << 4));
-        float4 v = ld_cluster4(cluster_addr(from, 0));
-#pragma unroll
-        for (int q = 1; q < 8; ++q)
-          if (q < a.split) {
-            const float4 u = ld_cluster4(cluster_addr(from, (uint32_t)q));
-            v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
-          }
-        const int n = n0 + 4 * lane;
-        const float* b = a.out.bias;
-        if (a.out.vec) {
-          if (n < a.out.n) f8_put4(a.out, v, b ? make_float4(b[n], b[n + 1], b[n + 2], b[n + 3]) : make_float4(0.f, 0.f, 0.f, 0.f), m0 + r, n);
-        } else {
-          const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (n + i < a.out.n) f8_put(a.out, e[i], b ? b[n + i] : 0.f, m0 + r, n + i);
-        }
-      }
+      if (a.split == 2) f8_join<XR, 2>(a.out, sm, rank, warp, m0, n0);
+      else if (a.split == 4) f8_join<XR, 4>(a.out, sm, rank, warp, m0, n0);
+      else f8_join<XR, 8>(a.out, sm, rank, warp, m0, n0);
+    } else {
+      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     }
     __syncwarp();
-    cluster_sync();  // the others may still read
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the others may still read
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -830,12 +859,36 @@ int launch_pair(fb200_device* dev, const F8Job& j) {
                       j.w->map64, xmap);
 }
 
+// The kernel, by the number of rows and a small cost model in microseconds (fitted to the times below, which hold for products one after
+// the other over weights that come from HBM):
+//  * up to 16 and up to 32 rows: the kernel for few rows, K split as far as the CTAs run at once and have four blocks each. One row,
+//    4096 x 14336: 32 us unsplit, 20, 13.7 and 12.0 split by 2, 4 and 8; 28672 x 4096: 20.1 unsplit, 25.6 by 2 (two rounds). 12 rows of
+//    4096 x 14336: 12.3, with the kernel for some rows 14.3;
+//  * above, single CTAs with 64 or 128 rows: a round takes 0.28 or 0.31 a block and 3 more, a split 2 more. By 8 it is slower (16 clusters of
+//    8 do not run at once: 64 rows of 4096 x 4096 8.6 us by 4, 17.8 by 8);
+//  * against pairs: a round takes 0.27 (128 weight rows) or 0.42 (256) a block and 1.5 more, 3.5 around them. 512 rows of 4096 x 4096: 13.6 us
+//    on single CTAs, 14.3 on pairs; 1024 of 6144 x 4096: 38.2 on single CTAs, 33.4 on pairs of 256, 35.1 of 128.
 int f8_product(fb200_device* dev, const F8Job& j) {
   const int m = j.out.m, n_tiles = (j.out.n + 127) / 128;
-  int rows = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128, split = 1, pair = 0;
-  const int tiles = n_tiles * ((m + rows - 1) / rows);
-  while (split < 8 && tiles * split * 2 <= dev->sm_count * (rows <= 32 ? 2 : 1) && j.kblocks >= split * 4) split *= 2;
-  if (m > 256) pair = 256;
+  int rows = m <= 16 ? 16 : 32, split = 1, pair = 0;
+  if (m <= 32) {
+    while (split < 8 && n_tiles * split * 2 <= dev->sm_count * 2 && j.kblocks >= split * 4) split *= 2;
+  } else {
+    double best = 1e30;
+    for (int r = 64; r <= 128; r *= 2)
+      for (int c = 1; c <= 4 && (c == 1 || j.kblocks >= c * 2); c *= 2) {
+        const long long tiles = (long long)n_tiles * ((m + r - 1) / r);
+        const int room = c == 4 ? dev->sm_count * 33 / 148 : dev->sm_count / c;  // clusters that run at once
+        const double cost = (double)((tiles + room - 1) / room) * ((j.kblocks + c - 1) / c * (r == 64 ? 0.28 : 0.31) + 3.0) + (c > 1 ? 2.0 : 0.0);
+        if (cost < best) best = cost, rows = r, split = c;
+      }
+    for (int nw = 128; nw <= 256; nw *= 2) {
+      const long long items = (long long)((j.out.n + nw - 1) / nw) * ((m + 255) / 256);
+      const int room = dev->sm_count / 2;
+      const double cost = (double)((items + room - 1) / room) * (j.kblocks * (nw == 128 ? 0.27 : 0.42) + 1.5) + 3.5;
+      if (cost < best) best = cost, pair = nw;
+    }
+  }
   // FB200_F8_TILE (tests, tuning; read per call): "ROWS,SPLIT" activation rows (16, 32, 64, 128) and ranges of K of the kernels on single
   // CTAs, "pair,NW" pairs with 128 or 256 weight rows; what there is not leaves the choice to the rule
   if (const char* cfg = getenv("FB200_F8_TILE")) {
