@@ -221,8 +221,9 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
   const uint32_t tmem = *tmem_slot;
   pdl_launch_dependents_small();  // behind the allocation: a dependent must not take columns that this grid still waits for
   // The cluster meets twice: everybody has started, so that partial sums may be sent, and (behind the sending) everybody has sent, so that
-  // nobody leaves while something may still come
-  if (a.split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  // nobody leaves while something may still come. Relaxed arrivals: the barriers' set-up is fenced above, and what is sent is counted by its
+  // receiver (a release took 1000 cycles each time).
+  if (a.split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
   if (warp < F::EPI_WARPS) {
     // ---- epilogue: warp w reads TMEM lanes 32 w .. = weight rows
@@ -305,7 +306,7 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
         for (int j = 0; j < BM; j += 2) st_cluster2(cluster_addr(mine, j / 2), acc[j / 2], cluster_addr(joined, j / 2));
       }
       __syncwarp();
-      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+      asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
       if (f_wait(joined, 0, dead, a.status) && n < a.out.n) {
         for (int j = 0; j < per && m0 + rank * per + j < a.out.m; ++j) {
           const float* from = part + tid * per + j;
@@ -357,7 +358,7 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
   if (warp >= F::EPI_WARPS && a.split > 1) {
     __syncwarp();
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
   __syncwarp();
@@ -623,7 +624,7 @@ f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // the barriers' set-up is fenced
   if (warp == 0) pair_tmem_alloc(smem_u32(tmem_slot), P::TMEM);
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 
