@@ -15,6 +15,7 @@
 #include <type_traits>
 
 #include "qgemv_common.cuh"
+#include "state_columns.cuh"
 
 namespace {
 
@@ -70,21 +71,20 @@ __device__ __forceinline__ Piece<T, E> f8_load(const T* row, int c, int n, bool 
   return r;
 }
 
-// The largest magnitude of a lane's values as f32 bits; these order magnitudes, with what is not finite above all. 16-bit values are
-// compared two at a time as they are.
+// The largest magnitude of a lane's values as f32 bits; these order magnitudes, with what is not finite above all. f32 values are compared
+// three at a time (a NaN wins), 16-bit values two at a time as they are.
 template <int E>
 __device__ __forceinline__ uint32_t f8_top(const float (&v)[E]) {
-  uint32_t top = 0;
+  float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < E; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  return top;
+  for (int i = 0; i < E; i += 2) asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(v[i]), "f"(v[i + 1]));
+  return __float_as_uint(top) & 0x7FFFFFFFu;
 }
 template <typename T, int E>
 __device__ __forceinline__ uint32_t f8_top_packed(const Piece<T, E>& r) {
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < Piece<T, E>::WORDS; ++i) top = sizeof(T) == 4 ? max(top, r.w[i] & 0x7FFFFFFFu) : __vmaxu2(top, r.w[i] & 0x7FFF7FFFu);
-  if (sizeof(T) == 4) return top;
+  for (int i = 0; i < Piece<T, E>::WORDS; ++i) top = __vmaxu2(top, r.w[i] & 0x7FFF7FFFu);
   const uint32_t one = max(top >> 16, top & 0xFFFFu);
   return std::is_same<T, __half>::value ? __float_as_uint(__half2float(__ushort_as_half((unsigned short)one))) : one << 16;
 }
@@ -112,9 +112,10 @@ __device__ __forceinline__ void f8_emit(const float (&v)[E], uint32_t top, int c
   if ((threadIdx.x & (LANES - 1)) == 0) scale_row[c / F8_BLOCK] = finite ? f8_quotient(a, F8_TOP, 1.0f / F8_TOP) : nan;
   uint32_t q[E / 4];
 #pragma unroll
-  for (int i = 0; i < E / 4; ++i)
-    q[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[4 * i] * r, v[4 * i + 1] * r), __NV_SATFINITE, __NV_E4M3) |
-           (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2] * r, v[4 * i + 3] * r), __NV_SATFINITE, __NV_E4M3) << 16;
+  for (int i = 0; i < E / 4; ++i) {
+    const float2 lo = mul2(make_float2(v[4 * i], v[4 * i + 1]), make_float2(r, r)), hi = mul2(make_float2(v[4 * i + 2], v[4 * i + 3]), make_float2(r, r));
+    q[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(lo, __NV_SATFINITE, __NV_E4M3) | (uint32_t)__nv_cvt_float2_to_fp8x2(hi, __NV_SATFINITE, __NV_E4M3) << 16;
+  }
   if (c + E <= n) {  // rows of codes begin on 16 bytes
     if (E == 16) *reinterpret_cast<uint4*>(code_row + c) = make_uint4(q[0], q[1], q[E / 4 - 2], q[E / 4 - 1]);
     else *reinterpret_cast<uint2*>(code_row + c) = make_uint2(q[0], q[1]);
@@ -123,7 +124,8 @@ __device__ __forceinline__ void f8_emit(const float (&v)[E], uint32_t top, int c
   }
 }
 
-// With the fast exponential (2 + 1.2 |g| units of its last place) and quotient (2 units): a code keeps four bits
+// silu(g) u = g u / (1 + exp(-g)), with the fast exponential (2 + 1.2 |g| units of its last place) and quotient (2 units): a code keeps
+// four bits
 __device__ __forceinline__ float f8_silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
 // Blocks by themselves: a warp takes STEPS x 32 x PER_LANE columns of a row, `wpr` warps stand side by side in a row. Its pieces
@@ -164,7 +166,7 @@ quantize_f8_kernel(const T* x, size_t ldx, const T* gate, size_t ldg, bool vec, 
 #pragma unroll
       for (int i = 0; i < E; ++i) v[i] = f8_silu_mul(g[i], v[i]);
     }
-    f8_emit(v, GATED ? f8_top(v) : f8_top_packed(xs[s]), c0 + s * SPAN, n, code_row, scale_row);
+    f8_emit(v, GATED || sizeof(T) == 4 ? f8_top(v) : f8_top_packed(xs[s]), c0 + s * SPAN, n, code_row, scale_row);
   }
 }
 
