@@ -265,7 +265,8 @@ FB200_API int fb200_sample(fb200_device* dev, const float* logits_dev, size_t ro
  * nearest even, both quotients in f32. A block with an infinity or a NaN gets NaN for its scale and all its codes.
  * Inputs are F32, F16 or BF16 (`type`), rows `ldx` .. elements apart; arithmetic is f32. Outputs may not overlap inputs, unless said so.
  * FB200_ERR_UNSUPPORTED_DTYPE for other types, FB200_ERR_INVALID_SHAPE for rows that overlap or are not aligned, for 2^31 rows or more
- * and for more than 2^27 columns. Zero rows or columns: nothing is written. */
+ * and for more than 2^27 columns. Zero rows or columns: nothing is written. Nothing here allocates or waits but the making of a matrix; the
+ * first launch of a kernel sets it up and loads its code, so make a call of the same sizes before a stream capture. */
 FB200_API int fb200_quantize_f8(fb200_device* dev, const void* x_dev, size_t ldx, uint32_t type, size_t rows, size_t n, uint8_t* codes_dev,
                                 size_t ld, float* scales_dev);
 /* The same of silu(gate) * up, the hidden row of a gated feed-forward (gate and up may be halves of the same rows). */
@@ -290,7 +291,8 @@ FB200_API int fb200_f8matrix_shape(const fb200_f8matrix* w, uint64_t* n_out, uin
 /* y[M, N] = x[M, K] . W^T (+ epilogue), y contiguous, F32, F16 or BF16 (`y_type`), rounded once. x is M rows of K codes and their scales.
  * The products of a block of 128 are summed by the tensor cores, the blocks under (x scale) x (W scale) in f32. Epilogues:
  * FB200_EPI_RESIDUAL and FB200_EPI_BIAS as in fb200_q_mat_mul (r1, r2 f32; an f32 y may be r1 or r2); no FB200_EPI_SWIGLU
- * (FB200_ERR_UNSUPPORTED_DTYPE). Results do not depend on timing; they may differ in the last bits between numbers of rows. */
+ * (FB200_ERR_UNSUPPORTED_DTYPE). M up to 2^27. Results do not depend on timing; they may differ in the last bits between numbers of
+ * rows. A row whose codes or scales are not finite, and a column whose weights are not, leaves the others as they are. */
 FB200_API int fb200_f8_mat_mul(fb200_device* dev, const uint8_t* codes_dev, size_t ld, const float* scales_dev, size_t m,
                                const fb200_f8matrix* w, uint32_t y_type, void* y_dev, const fb200_epilogue* epilogue);
 

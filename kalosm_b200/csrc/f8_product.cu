@@ -7,9 +7,16 @@
 // one row of a 128-byte swizzled operand and four MMAs. The outer sum is kept in f32 registers: the epilogue warps take each block's
 // accumulator out of tensor memory while the tensor cores fill the next one, and add it under its scale.
 //
-// f8_few_kernel (weights in the M role): 128 weight rows by BM activation rows per CTA, K split over a cluster whose CTAs join their sums
-// through distributed shared memory in the order of their ranks. Bound: HBM (N K bytes) for few rows.
-// f8_pair_kernel (activations in the M role): CTA pairs, 256 activation rows by NW weight rows. Bound: tensor cores.
+// Three kernels, by the number of rows (f8_product has the rule and what it was measured on):
+//  * f8_few_kernel, up to 32: 128 weight rows (in the M role) by 16 or 32 activation rows per CTA, K split over a cluster whose CTAs send
+//    their sums to their owner through distributed shared memory. Bound: HBM, N K bytes. One row of 4096 x 4096: 5.4 us (3.1 TB/s, launches
+//    one after the other; half of it is set-up and the hand-over of sums), of 28672 x 4096: 20.1 us (5.8 TB/s);
+//  * f8_some_kernel, to a few hundred: 64 or 128 activation rows (in the M role, so that a thread has one row and one scale) by 128 weight
+//    rows, K split over clusters of up to four. Bound: HBM, then what an SM takes in from L2 (94 GB/s measured). 128 rows of
+//    4096 x 14336: 16.4 us (3.7 TB/s, 0.92 PFLOP/s);
+//  * f8_pair_kernel: CTA pairs, 256 activation rows by 128 or 256 weight rows, persistent. Bound: what the SMs take in from L2 (32 KB per pair
+//    tile and block and SM: without its MMAs the kernel takes 0.9 of its time) and the power limit. 8192 rows of 28672 x 4096: 831 us
+//    (2.3 PFLOP/s), 930 us at the 1.4 GHz that 950 W leave in a long run.
 // Every wait is bounded (2^22 polls): one that gives up sets the device status word and a flag that makes the other roles leave; copies
 // and MMAs in flight are waited for, TMEM is released on every path.
 #include <cstdlib>
@@ -157,7 +164,7 @@ struct Few {
   static constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(BM >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 };
 
-struct FewArgs {
+struct SplitArgs {
   const float *sx, *sw;
   F8Out out;
   int kblocks, m_tiles, split;
@@ -176,7 +183,7 @@ __device__ __forceinline__ void st_cluster2(uint32_t addr, float2 a, uint32_t ba
 
 template <int BM>
 __global__ void __launch_bounds__(Few<BM>::THREADS, 2)
-f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
+f8_few_kernel(const SplitArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
   using F = Few<BM>;
   extern __shared__ uint8_t sm_raw[];
   // the same offset in every CTA of the cluster: their dynamic shared memory starts at the same address
@@ -338,6 +345,7 @@ f8_few_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const _
     }
   } else {
     // ---- MMA issuer
+    pdl_wait();  // the limit of its waits does not count the kernel in front
     const uint64_t adesc0 = x_desc_rows(smem_u32(sm)), bdesc0 = x_desc_rows(smem_u32(sm) + F8_A_BYTES);
     int st = 0, buf = 0;
     uint32_t parity = 0, round = 0;
@@ -436,7 +444,7 @@ __device__ __forceinline__ void f8_join(const F8Out& o, const uint8_t* sm, int r
 
 template <int XR>
 __global__ void __launch_bounds__(Some<XR>::THREADS, 1)
-f8_some_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
+f8_some_kernel(const SplitArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
   using F = Some<XR>;
   extern __shared__ uint8_t sm_raw[];
   // the same offset in every CTA of the cluster: their dynamic shared memory starts at the same address
@@ -526,6 +534,7 @@ f8_some_kernel(const FewArgs a, const __grid_constant__ CUtensorMap wmap, const 
     }
   } else if (warp > F::EPI_WARPS) {
     // ---- two MMA issuers, every other block each
+    pdl_wait();
     const uint64_t adesc0 = x_desc_rows(smem_u32(sm)), bdesc0 = x_desc_rows(smem_u32(sm) + XR * 128);
     const int which = warp - F::EPI_WARPS - 1;
     int st = which;
@@ -756,6 +765,7 @@ f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const
     const uint32_t which = warp - PAIR_EPI_WARPS - 1, part = P::PARTS == 2 ? which : 0, step = 2 / P::PARTS;
     const uint32_t blocks = (uint32_t)((items - pair + npairs - 1) / npairs) * (uint32_t)a.kblocks;
     if (rank == 0) {
+      pdl_wait();
       const uint64_t adesc0 = x_desc_rows(smem_u32(sm)), bdesc0 = x_desc_rows(smem_u32(sm) + F8_A_BYTES) + part * (64 * 128 >> 4);
       uint32_t s = P::PARTS == 2 ? 0 : which, parity = 0;
       for (uint32_t k = s; k < blocks; k += step) {
@@ -770,8 +780,8 @@ f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const
         if ((s += step) >= P::STAGES) { s -= P::STAGES; parity ^= 1u; }
       }
       pair_commit(drained);
+      x_drain(drained, 0);  // the odd CTA learns of it at the last meeting
     }
-    x_drain(drained, 0);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   }
@@ -809,7 +819,7 @@ int launch_split(fb200_device* dev, const F8Job& j, K kern, int rows, int thread
   CUtensorMap xmap;
   if (!fb200_make_map_2d_bytes(&xmap, j.x, j.w->k, (uint64_t)j.out.m, j.ld, (uint32_t)rows))
     return fb200_fail(dev, FB200_ERR_CUDA, "f8_mat_mul: tensor map refused (x %d rows every %zu bytes)", j.out.m, j.ld);
-  const FewArgs a = {j.sx, j.w->scales, j.out, j.kblocks, (j.out.m + rows - 1) / rows, split, dev->status};
+  const SplitArgs a = {j.sx, j.w->scales, j.out, j.kblocks, (j.out.m + rows - 1) / rows, split, dev->status};
   const long long ctas = (long long)a.m_tiles * ((j.out.n + 127) / 128) * split;
   if (ctas > 0x7FFFFFFF) return fb200_fail(dev, FB200_ERR_INVALID_SHAPE, "f8_mat_mul: %d x %d outputs are too many", j.out.m, j.out.n);
   cudaLaunchConfig_t cfg = {};
@@ -977,6 +987,7 @@ int fb200_f8matrix_from_device(fb200_device* dev, const uint64_t* shape, int ran
   // products fetch the codes without waiting for the kernel in front of them: what writes them has to be done
   const cudaError_t e = cudaStreamSynchronize(dev->stream);
   rc = e == cudaSuccess ? make_maps(dev, w) : fb200_fail(dev, FB200_ERR_CUDA, "F8Matrix: %s", cudaGetErrorString(e));
+  if (e != cudaSuccess) cudaGetLastError();
   if (rc) {
     delete w;
     return rc;
