@@ -599,6 +599,8 @@ class F8Rows:
 
     def __init__(self, device: Device, shape: Sequence[int], codes: Tensor = None, scales: Tensor = None):
         self.device, self.shape = device, tuple(int(s) for s in shape)
+        if not self.shape:
+            raise FusorError(ERR_INVALID_SHAPE, "rows need a shape of at least one axis")
         self.rows, n = _rows_of(self.shape), self.shape[-1]
         self.blocks = -(-n // 128)
         self.codes = Tensor(device, (self.rows, -(-n // 16) * 16), np.uint8) if codes is None else codes
@@ -635,8 +637,10 @@ class F8Rows:
                                                 f"(got {out.dtype}, {out.nbytes} bytes)")
         self.codes._require_f32("r1", r1, n if epilogue == EPI_BIAS else m * n)
         self.codes._require_f32("r2", r2, m * n)
-        ep = _Epilogue(epilogue, r1.ptr if r1 is not None else None, r2.ptr if r2 is not None else None)
-        d._check(d.lib.fb200_f8_mat_mul(d.h, self.codes.ptr, self.ld, self.scales.ptr, m, w.h, out_type, out.ptr, C.byref(ep)))
+        ep = None
+        if epilogue != EPI_NONE or r1 is not None or r2 is not None:
+            ep = C.byref(_Epilogue(epilogue, r1.ptr if r1 is not None else None, r2.ptr if r2 is not None else None))
+        d._check(d.lib.fb200_f8_mat_mul(d.h, self.codes.ptr, self.ld, self.scales.ptr, m, w.h, out_type, out.ptr, ep))
         return out
 
 

@@ -58,6 +58,7 @@ def test_rows_are_checked():
                           (t((6, 144), np.uint8), t((6, 1), np.float32)), (t((6, 144), np.uint8), t((6, 2), np.float16)),
                           (t((6, 144), np.uint8, _fake()), t((6, 2), np.float32)), (t((6, 144), np.uint8), t((6, 2), np.float32, _fake()))]:
         _refused(kb.ERR_INVALID_SHAPE, lambda: kb.F8Rows(dev, (2, 3, 130), codes, scales))
+    _refused(kb.ERR_INVALID_SHAPE, lambda: kb.F8Rows(dev, ()))
     _refused(kb.ERR_INVALID_SHAPE, lambda: kb.F8Matrix.from_tensors(t((6, 144), np.int8), t((1, 2), np.float32)))
     _refused(kb.ERR_INVALID_SHAPE, lambda: kb.F8Matrix.from_tensors(t((6, 144), np.uint8), t((1, 2), np.float32), 145))
     _refused(kb.ERR_INVALID_SHAPE, lambda: kb.F8Matrix.from_tensors(t((6, 144), np.uint8), t((6, 2), np.float32), 130))

@@ -276,7 +276,8 @@ def test_product_epilogues(dev, monkeypatch, kind, epilogue, second, tile, m, n)
     run_product(dev, np.random.default_rng(n + m), m, n, 400, kind, epilogue, second)
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (12, 4096, 14336), (1, 28672, 4096), (100, 6144, 4096), (1024, 1024, 2048)])
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (12, 4096, 14336), (1, 28672, 4096), (100, 6144, 4096), (1024, 1024, 2048), (5, 300, 70000),
+                                   (2100, 2700, 700)])
 def test_product_model_sizes(dev, m, n, k):
     run_product(dev, np.random.default_rng(k), m, n, k, "bf16", kb.EPI_RESIDUAL)
 
@@ -389,6 +390,61 @@ def test_refusals(dev):
     assert other.lib.fb200_f8_mat_mul(other.h, c.ptr, 256, s.ptr, 4, w.h, kb.F32, p, None) == kb.ERR_DEVICE_MISMATCH
     other.close()
     assert dev.status() == 0
+
+
+# ---- far rows -----------------------------------------------------------------------------------------------------------
+
+def _part(t, byte, shape, kind):
+    return kb.Tensor(t.device, shape, kind, ptr=t.ptr + byte)
+
+
+def _put(t, byte, a):
+    a = np.ascontiguousarray(a)
+    t.device._check(t.device.lib.fb200_upload(t.device.h, t.ptr + byte, a.ctypes.data, a.nbytes))
+
+
+def test_rows_behind_two_to_the_32(dev):
+    """Rows whose elements, and bytes, lie further than 32 bits from the first: codes of bf16 rows, norms in place, outputs of a product."""
+    rng = np.random.default_rng(31)
+    rows, n = 270000, 16384
+    look = [0, 131071, 131072, 262143, 262144, rows - 1]  # around 2^31 and 2^32 elements
+    a, v = F.held("bf16", spread(rng, len(look), n))
+    x, codes, scales = dev.empty((rows, n), np.uint16), dev.empty((rows, n), np.uint8), dev.empty((rows, n // 128))
+    w = dev.tensor(np.ones(n, dtype=np.float32))
+
+    def write():
+        x.fill_bytes(0)
+        for i, r in enumerate(look):
+            _put(x, r * n * 2, a[i])
+
+    def read():
+        c = np.stack([_part(codes, r * n, (n,), np.uint8).as_slice() for r in look])
+        return c, np.stack([_part(scales, r * (n // 128) * 4, (n // 128,), np.float32).as_slice() for r in look]).astype(np.float64)
+
+    write()
+    out = kb.F8Rows(dev, (rows, n), codes, scales)
+    dev.quantize_f8(x, out=out)
+    F.check_rows(*read(), v, np.zeros_like(v))
+    dev.rms_norm_f8(x, w, EPS, residual=x, sum_out=x, out=out)
+    s, y, dy = rms_norm(v, v, 1.0, None, EPS, 69)
+    F.check_rows(*read(), y, dy)
+    got = np.stack([F.bf16(_part(x, r * n * 2, (n,), np.uint16).as_slice()) for r in look])
+    assert np.array_equal(got, s)  # twice a bf16 value
+    del x, codes, scales, out
+
+    m, n, k = 160000, 28000, 130
+    look = [0, 76695, 76696, 153390, 153391, m - 1]  # around 2^31 and 2^32 outputs
+    cx, sx, cw, sw = operands(rng, len(look), n, k)
+    all_codes, all_scales = dev.empty((m, 144), np.uint8), dev.empty((m, 2))
+    all_codes.fill_bytes(0)
+    all_scales.fill_bytes(0)
+    for i, r in enumerate(look):
+        _put(all_codes, r * 144, cx[i])
+        _put(all_scales, r * 8, sx[i])
+    y = kb.F8Rows(dev, (m, k), all_codes, all_scales).f8_mat_mul(kb.F8Matrix.from_raw_bytes(dev, (n, k), cw, sw), kb.BF16)
+    want, bound = F.product(cx, sx, cw, sw)
+    check("bf16", np.stack([_part(y, r * n * 2, (n,), np.uint16).as_slice() for r in look]), want, bound)
+    assert not _part(y, 76697 * n * 2, (n,), np.uint16).as_slice().any() and not _part(y, 153392 * n * 2, (n,), np.uint16).as_slice().any()
 
 
 # ---- together -----------------------------------------------------------------------------------------------------------
