@@ -261,6 +261,15 @@ def test_product_tiles(dev, monkeypatch, tile, m, n, k):
     run_product(dev, np.random.default_rng(m + n + k), m, n, k)
 
 
+@pytest.mark.parametrize("m,n,k", [(300, 256 * 40, 300), (300, 256 * 40 - 77, 1000), (256, 256 * 75, 128), (513, 256 * 50 + 3, 130), (256, 256 * 111, 900)])
+def test_product_several_tiles_per_pair(dev, monkeypatch, m, n, k):
+    """More tiles than pairs, so that a pair goes from tile to tile (148 SMs: 80, 80, 75, 153 and 111 tiles of 256 x 256 on 74 pairs)."""
+    for tile in ("pair,256", "pair,128"):
+        monkeypatch.setenv("FB200_F8_TILE", tile)
+        run_product(dev, np.random.default_rng(n), m, n, k, "bf16")
+    run_product(dev, np.random.default_rng(n), m, n, k, "f32", kb.EPI_BIAS)
+
+
 @pytest.mark.parametrize("m", [1, 2, 8, 13, 16, 17, 32, 33, 64, 65, 128, 129, 200, 256, 257, 700])
 @pytest.mark.parametrize("n,k", [(384, 512), (1000, 3000)])
 def test_product_rows(dev, m, n, k):
