@@ -571,8 +571,7 @@ f8_some_kernel(const SplitArgs a, const __grid_constant__ CUtensorMap wmap, cons
     cluster_sync();
     if (warp < F::EPI_WARPS) {
       if (a.split == 2) f8_join<XR, 2>(a.out, sm, rank, warp, m0, n0);
-      else if (a.split == 4) f8_join<XR, 4>(a.out, sm, rank, warp, m0, n0);
-      else f8_join<XR, 8>(a.out, sm, rank, warp, m0, n0);
+      else f8_join<XR, 4>(a.out, sm, rank, warp, m0, n0);
     } else {
       asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     }
@@ -875,7 +874,7 @@ int launch_pair(fb200_device* dev, const F8Job& j) {
 //  * up to 16 and up to 32 rows: the kernel for few rows, K split as far as the CTAs run at once and have four blocks each. One row,
 //    4096 x 14336: 32 us unsplit, 20, 13.7 and 12.0 split by 2, 4 and 8; 28672 x 4096: 20.1 unsplit, 25.6 by 2 (two rounds). 12 rows of
 //    4096 x 14336: 12.3, with the kernel for some rows 14.3;
-//  * above, single CTAs with 64 or 128 rows: a round takes 0.28 or 0.31 a block and 3 more, a split 2 more. By 8 it is slower (16 clusters of
+//  * above, single CTAs with 64 or 128 rows: a round takes 0.28 or 0.31 a block and 3 more, a split 2 more. By 8 it was slower (16 clusters of
 //    8 do not run at once: 64 rows of 4096 x 4096 8.6 us by 4, 17.8 by 8);
 //  * against pairs: a round takes 0.27 (128 weight rows) or 0.42 (256) a block and 1.5 more, 3.5 around them. 512 rows of 4096 x 4096: 13.6 us
 //    on single CTAs, 14.3 on pairs; 1024 of 6144 x 4096: 38.2 on single CTAs, 33.4 on pairs of 256, 35.1 of 128.
@@ -900,14 +899,14 @@ int f8_product(fb200_device* dev, const F8Job& j) {
       if (cost < best) best = cost, pair = nw;
     }
   }
-  // FB200_F8_TILE (tests, tuning; read per call): "ROWS,SPLIT" activation rows (16, 32, 64, 128) and ranges of K of the kernels on single
-  // CTAs, "pair,NW" pairs with 128 or 256 weight rows; what there is not leaves the choice to the rule
+  // FB200_F8_TILE (tests, tuning; read per call): "ROWS,SPLIT" activation rows (16, 32, 64, 128) and ranges of K (8 with 16 or 32 rows
+  // only) of the kernels on single CTAs, "pair,NW" pairs with 128 or 256 weight rows; what there is not leaves the choice to the rule
   if (const char* cfg = getenv("FB200_F8_TILE")) {
     int frows, fsplit;
     if (sscanf(cfg, "pair,%d", &frows) == 1) {
       if (frows == 128 || frows == 256) pair = frows;
     } else if (sscanf(cfg, "%d,%d", &frows, &fsplit) == 2 && (frows == 16 || frows == 32 || frows == 64 || frows == 128) &&
-               (fsplit == 1 || fsplit == 2 || fsplit == 4 || fsplit == 8)) {
+               (fsplit == 1 || fsplit == 2 || fsplit == 4 || (fsplit == 8 && frows <= 32))) {
       rows = frows, split = fsplit, pair = 0;
     }
   }

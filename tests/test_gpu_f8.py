@@ -110,6 +110,20 @@ def test_silu_mul(dev, kind, rows, n):
     assert np.array_equal(apart.scales.as_slice(), both.scales.as_slice())
 
 
+def test_silu_mul_strided(dev):
+    """Gate and up in rows of their own lengths, at addresses that allow no wide loads; with n = 1 too."""
+    rng = np.random.default_rng(17)
+    for kind, n in [("f32", 1000), ("f16", 515), ("bf16", 1), ("bf16", 2048)]:
+        rows, ldg, ldu = 5, n + 3, n + 16
+        (ag, g), (au, u) = F.held(kind, rng.standard_normal((rows + 1, ldg))), F.held(kind, rng.standard_normal((rows + 1, ldu)))
+        tg, tu = upload(dev, ag), upload(dev, au)
+        codes, scales, ld = new_rows(dev, rows, n, 1)
+        dev._check(dev.lib.fb200_silu_mul_f8(dev.h, tg.ptr + ag.itemsize, ldg, tu.ptr + 8 * au.itemsize, ldu, TYPES[kind], rows, n, codes.ptr, ld, scales.ptr))
+        at = np.arange(rows)[:, None]
+        v, dv = silu_mul(g.reshape(-1)[1 + at * ldg + np.arange(n)], u.reshape(-1)[8 + at * ldu + np.arange(n)])
+        F.check_rows(*result(codes, scales, rows, n), v, dv)
+
+
 def test_silu_mul_far_gates(dev):
     g = np.array([[-1e30, -200, -104, -88.5, -60, -20, 0, 20, 60, 88.5, 200, 1e30]], dtype=np.float32)
     u = np.array([[1, 1, 1, -1, 1, 1, 1, 1, 1, -1, 1, 1e-28]], dtype=np.float32)
@@ -205,7 +219,7 @@ def test_rms_norm_of_zero_and_not_finite_rows(dev):
 
 # ---- the product --------------------------------------------------------------------------------------------------------
 
-TILES = ["16,1", "16,2", "16,4", "16,8", "32,1", "32,4", "32,8", "64,1", "64,2", "64,8", "128,1", "128,2", "128,4", "128,8", "pair,128", "pair,256"]
+TILES = ["16,1", "16,2", "16,4", "16,8", "32,1", "32,4", "32,8", "64,1", "64,2", "64,4", "128,1", "128,2", "128,4", "pair,128", "pair,256"]
 
 
 def operands(rng, m, n, k):
@@ -325,6 +339,29 @@ def test_product_over_borrowed_codes_and_into_its_residual(dev):
         stream = dev.tensor(r)
         device_rows(dev, x, xs, 3).f8_mat_mul(mat, epilogue=kb.EPI_RESIDUAL, r1=stream, out=stream)
         check("f32", stream.as_slice(), y + r, bound + F.U * (np.abs(y) + bound + np.abs(r)))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("tile,m", [("16,2", 9), ("64,2", 40), ("128,1", 140), ("pair,256", 300)])
+def test_product_into_unaligned_rows(dev, monkeypatch, kind, tile, m):
+    """Outputs and residuals one element behind an aligned address, in a width that would allow wide stores."""
+    monkeypatch.setenv("FB200_F8_TILE", tile)
+    rng = np.random.default_rng(m)
+    n, k = 256, 384
+    x, xs, w, ws = operands(rng, m, n, k)
+    y, bound = F.product(x, xs, w, ws)
+    r = rng.standard_normal(m * n + 1).astype(np.float32)
+    size = 4 if kind == "f32" else 2
+    out, t, rows = dev.empty((m * n + 2,), {"f32": np.float32, "f16": np.float16, "bf16": np.uint16}[kind]), dev.tensor(r), device_rows(dev, x, xs)
+    mat = kb.F8Matrix.from_raw_bytes(dev, (n, k), w, ws)
+    for res in (False, True):
+        out.fill_bytes(GUARD)
+        ep = kb._Epilogue(kb.EPI_RESIDUAL, t.ptr + 4, None)
+        dev._check(dev.lib.fb200_f8_mat_mul(dev.h, rows.codes.ptr, rows.ld, rows.scales.ptr, m, mat.h, TYPES[kind], out.ptr + size, C.byref(ep) if res else None))
+        got = out.as_slice()
+        assert np.all(got[[0, -1]].view(np.uint8) == GUARD)
+        add = r[1:].reshape(m, n).astype(np.float64) if res else 0.0
+        check(kind, got[1:-1].reshape(m, n), y + add, bound + F.U * (np.abs(y) + bound + np.abs(add)))
 
 
 def test_no_rows(dev):
