@@ -50,62 +50,102 @@ struct F8Out {
   int pack;  // 16-bit y without residual or bias, eight columns aligned: rounded before they are turned
 };
 
-// The output (m, n): v + its bias + the residuals, rounded once
-__device__ __forceinline__ void f8_put(const F8Out& o, float v, float bias, int m, int n) {
-  const size_t at = (size_t)m * o.n + n;
-  v += bias;
-  if (o.r1) v += o.r1[at];
-  if (o.r2) v += o.r2[at];
-  if (o.type == FB200_F32) reinterpret_cast<float*>(o.y)[at] = v;
-  else if (o.type == FB200_BF16) reinterpret_cast<__nv_bfloat16*>(o.y)[at] = __float2bfloat16(v);
-  else reinterpret_cast<__half*>(o.y)[at] = __float2half(v);
-}
-
 constexpr int TURN_BYTES = 32 * 128;  // a warp's 32 rows x 128 bytes on their way out, 16-byte piece p of row r at place p ^ (r % 8)
 
+// Two outputs in 16 bits
 __device__ __forceinline__ uint32_t f8_pair(const F8Out& o, float2 v) {
   const __nv_bfloat162 b = __floats2bfloat162_rn(v.x, v.y);
   const __half2 h = __floats2half2_rn(v.x, v.y);
   return o.type == FB200_BF16 ? *reinterpret_cast<const uint32_t*>(&b) : *reinterpret_cast<const uint32_t*>(&h);
 }
-// Four neighbouring outputs
-__device__ __forceinline__ void f8_put4(const F8Out& o, float4 v, const float4& bias, int m, int n) {
-  const size_t at = (size_t)m * o.n + n;
-  v.x += bias.x; v.y += bias.y; v.z += bias.z; v.w += bias.w;
-  if (o.r1) { const float4 r = *reinterpret_cast<const float4*>(o.r1 + at); v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w; }
-  if (o.r2) { const float4 r = *reinterpret_cast<const float4*>(o.r2 + at); v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w; }
-  if (o.type == FB200_F32) {
-    *reinterpret_cast<float4*>(reinterpret_cast<float*>(o.y) + at) = v;
+// One output, and four neighbouring ones (o.vec), rounded; `at` counts elements
+__device__ __forceinline__ void f8_put(const F8Out& o, float v, size_t at) {
+  if (o.type == FB200_F32) reinterpret_cast<float*>(o.y)[at] = v;
+  else reinterpret_cast<uint16_t*>(o.y)[at] = (uint16_t)f8_pair(o, make_float2(v, 0.f));
+}
+__device__ __forceinline__ void f8_put4(const F8Out& o, const float4& v, size_t at) {
+  if (o.type == FB200_F32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(o.y) + at) = v;
+  else *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(o.y) + at) = make_uint2(f8_pair(o, make_float2(v.x, v.y)), f8_pair(o, make_float2(v.z, v.w)));
+}
+__device__ __forceinline__ float4 f8_add(const float4& a, const float4& b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
+// Columns n .. n + 3 of a vector of N or of a row of a matrix of N columns, zeros behind it
+__device__ __forceinline__ float4 f8_four(const float* p, int n, int N, bool vec) {
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (vec) {
+    if (n < N) v = *reinterpret_cast<const float4*>(p + n);
   } else {
-    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(o.y) + at) = make_uint2(f8_pair(o, make_float2(v.x, v.y)), f8_pair(o, make_float2(v.z, v.w)));
+    if (n < N) v.x = p[n];
+    if (n + 1 < N) v.y = p[n + 1];
+    if (n + 2 < N) v.z = p[n + 2];
+    if (n + 3 < N) v.w = p[n + 3];
+  }
+  return v;
+}
+
+// Asks L2 for a warp's part of the residuals, 32 rows from m0 and COLS columns from n0 on: it is added when the tile is done
+template <int COLS>
+__device__ __forceinline__ void f8_ask_residuals(const F8Out& o, int m0, int n0) {
+  const int m = m0 + (int)(threadIdx.x & 31);
+  if (m >= o.m) return;
+#pragma unroll
+  for (int c = 0; c < COLS; c += 32) {
+    if (n0 + c >= o.n) break;
+    const size_t at = (size_t)m * o.n + n0 + c;
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(o.r1 + at));
+    if (o.r2) asm volatile("prefetch.global.L2 [%0];" ::"l"(o.r2 + at));
   }
 }
 
-// Turned rows of 32 f32 columns to y, `rows` of them from m0 on; the lane's column is on the matrix
+// Turned rows of 32 f32 columns to y, `rows` of them from m0 on; the lane's column n is on the matrix. Residuals: eight rows at a time, all
+// loads, then all stores (y may be a residual, so that the compiler moves no load before a store): 4000 rows of 5001 x 700 to f32 took
+// 291 us a row at a time and take 83, without residuals 42. Batches cost the rows without residuals time (16 bits: 52 us instead of 44).
+template <bool RES>
 __device__ __forceinline__ void f8_rows_out(const F8Out& o, const uint8_t* turn, int rows, int m0, int n) {
-  const float bias = o.bias ? o.bias[n] : 0.f;
-  const uintptr_t from = reinterpret_cast<uintptr_t>(turn) + 4 * (threadIdx.x & 31);
+  const int lane = threadIdx.x & 31;
   const size_t first = (size_t)m0 * o.n + n;
-  const int size = o.type == FB200_F32 ? 4 : 2;
-  uint8_t* to = reinterpret_cast<uint8_t*>(o.y) + first * size;
-  const float *p1 = o.r1 + first, *p2 = o.r2 + first;
+  if (!RES) {
+    const float bias = o.bias ? o.bias[n] : 0.f;
+    const int size = o.type == FB200_F32 ? 4 : 2;
+    const uintptr_t from = reinterpret_cast<uintptr_t>(turn) + 4 * lane;
+    uint8_t* to = reinterpret_cast<uint8_t*>(o.y) + first * size;
 #pragma unroll 8
-  for (int r = 0; r < rows; ++r, to += (size_t)o.n * size) {
-    float v = *reinterpret_cast<const float*>((from ^ ((r & 7) << 4)) + r * 128) + bias;
-    if (o.r1) v += p1[(size_t)r * o.n];
-    if (o.r2) v += p2[(size_t)r * o.n];
-    if (size == 4) *reinterpret_cast<float*>(to) = v;
-    else *reinterpret_cast<uint16_t*>(to) = (uint16_t)f8_pair(o, make_float2(v, 0.f));
+    for (int r = 0; r < rows; ++r, to += (size_t)o.n * size) {
+      const float v = *reinterpret_cast<const float*>((from ^ ((r & 7) << 4)) + r * 128) + bias;
+      if (size == 4) *reinterpret_cast<float*>(to) = v;
+      else *reinterpret_cast<uint16_t*>(to) = (uint16_t)f8_pair(o, make_float2(v, 0.f));
+    }
+    return;
+  }
+  const float *p1 = o.r1 + first, *p2 = o.r2 + first;
+#pragma unroll 1
+  for (int r0 = 0; r0 < rows; r0 += 8) {
+    const bool all = r0 + 8 <= rows;
+    float v[8], e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const float*>(turn + (r0 + i) * 128 + (((lane >> 2) ^ i) << 4) + 4 * (lane & 3));
+#pragma unroll
+    for (int i = 0; i < 8; ++i, p1 += o.n) e[i] = all || r0 + i < rows ? *p1 : 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += e[i];
+    if (o.r2) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i, p2 += o.n) e[i] = all || r0 + i < rows ? *p2 : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += e[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (all || r0 + i < rows) f8_put(o, v[i], first + (size_t)(r0 + i) * o.n);
   }
 }
 
 // A warp's 32 rows from m0 on, COLS columns from n0 on, a row per thread, to y: turned in shared memory, so that a row's columns leave
 // together.
-template <int COLS>
+template <int COLS, bool RES>
 __device__ __forceinline__ void f8_store_rows(const F8Out& o, const float2 (&acc)[COLS / 2], uint8_t* turn, int m0, int n0) {
   const int lane = threadIdx.x & 31, rows = min(32, o.m - m0), n_end = o.n - n0;
   uint4* mine = reinterpret_cast<uint4*>(turn + lane * 128);
-  if (o.pack) {
+  if (!RES && o.pack) {
     uint16_t* to = reinterpret_cast<uint16_t*>(o.y) + (size_t)m0 * o.n + n0 + 8 * (lane & 7);
 #pragma unroll
     for (int c = 0; c < COLS / 64; ++c) {
@@ -126,6 +166,11 @@ __device__ __forceinline__ void f8_store_rows(const F8Out& o, const float2 (&acc
     }
     return;
   }
+  // o.vec: a lane has four columns of every fourth row. The residuals of four rows are in flight together, all loads ahead of the stores (y
+  // may be a residual, so that the compiler moves none): 8192 rows of 4096 x 4096 to f32 with one take 165 us, 4000 rows of 5000 x 700 take
+  // 57, one row at a time 125. Eight rows at a time spilled registers: 197 and 75 us.
+  const int n4 = n0 + 4 * (lane & 7);
+  const size_t at4 = (size_t)(m0 + (lane >> 3)) * o.n + n4;
 #pragma unroll
   for (int c = 0; c < COLS / 32; ++c) {
     if (32 * c >= n_end) break;
@@ -137,15 +182,38 @@ __device__ __forceinline__ void f8_store_rows(const F8Out& o, const float2 (&acc
     }
     __syncwarp();
     if (o.vec) {  // whole fours: N is a multiple of four then
-      const int n = n0 + 32 * c + 4 * (lane & 7);
-      if (n < o.n) {
-        const float4 bias = o.bias ? make_float4(o.bias[n], o.bias[n + 1], o.bias[n + 2], o.bias[n + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int r = lane >> 3; r < rows; r += 4)
-          f8_put4(o, *reinterpret_cast<const float4*>(turn + r * 128 + (((lane & 7) ^ (r & 7)) << 4)), bias, m0 + r, n);
+      if (n4 + 32 * c < o.n) {
+        const float4 bias = o.bias ? f8_four(o.bias, n4 + 32 * c, o.n, false) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int h = 0; h < 8; h += 4) {
+          const float *p1 = o.r1 + at4 + (size_t)(4 * h) * o.n + 32 * c, *p2 = o.r2 + at4 + (size_t)(4 * h) * o.n + 32 * c;
+          const int left = rows - 4 * h - (lane >> 3);
+          float4 v[4], e[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (RES && 4 * i < left) e[i] = *reinterpret_cast<const float4*>(p1 + (size_t)(4 * i) * o.n);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 4 * (h + i) + (lane >> 3);
+            v[i] = f8_add(*reinterpret_cast<const float4*>(turn + r * 128 + (((lane & 7) ^ (r & 7)) << 4)), bias);
+            if (RES && 4 * i < left) v[i] = f8_add(v[i], e[i]);
+          }
+          if (RES && o.r2) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (4 * i < left) e[i] = *reinterpret_cast<const float4*>(p2 + (size_t)(4 * i) * o.n);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (4 * i < left) v[i] = f8_add(v[i], e[i]);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (4 * i < left) f8_put4(o, v[i], at4 + (size_t)(4 * (h + i)) * o.n + 32 * c);
+        }
       }
     } else if (32 * c + lane < n_end) {
-      f8_rows_out(o, turn, rows, m0, n0 + 32 * c + lane);
+      f8_rows_out<RES>(o, turn, rows, m0, n0 + 32 * c + lane);
     }
   }
 }
@@ -252,6 +320,17 @@ f8_few_kernel(const SplitArgs a, const __grid_constant__ CUtensorMap wmap, const
     };
     pdl_wait();
     fetch(0);
+    // this thread's outputs and what is added to them, asked for ahead of the blocks: `per` rows from m1 on
+    const int n = nt * 128 + tid, per = BM / a.split, m1 = m0 + rank * per;
+    const bool on = n < a.out.n;
+    const float bias = a.out.bias && on ? a.out.bias[n] : 0.f;
+    float e1[BM], e2[BM];
+#pragma unroll
+    for (int j = 0; j < BM; ++j) {
+      const bool in = on && j < per && m1 + j < a.out.m;
+      e1[j] = in && a.out.r1 ? a.out.r1[(size_t)(m1 + j) * a.out.n + n] : 0.f;
+      e2[j] = in && a.out.r2 ? a.out.r2[(size_t)(m1 + j) * a.out.n + n] : 0.f;
+    }
     int buf = 0;
     uint32_t parity = 0;
     for (int i = 0; i < nkb; ++i) {
@@ -288,17 +367,13 @@ f8_few_kernel(const SplitArgs a, const __grid_constant__ CUtensorMap wmap, const
       }
       if (++buf == F::BUFS) { buf = 0; parity ^= 1u; }
     }
-    const int n = nt * 128 + tid;
-    const float bias = a.out.bias && n < a.out.n ? a.out.bias[n] : 0.f;
     if (a.split == 1) {
-      if (n < a.out.n)
 #pragma unroll
-        for (int j = 0; j < BM; ++j)
-          if (m0 + j < a.out.m) f8_put(a.out, j & 1 ? acc[j / 2].y : acc[j / 2].x, bias, m0 + j, n);
+      for (int j = 0; j < BM; ++j)
+        if (on && m1 + j < a.out.m) f8_put(a.out, (j & 1 ? acc[j / 2].y : acc[j / 2].x) + bias + e1[j] + e2[j], (size_t)(m1 + j) * a.out.n + n);
     } else {
       // The sums of the cluster's ranges of K: rank q gets activation rows BM q / split .. of all, [rank][weight row][activation row], and
       // adds them in the order of the ranks. (Fetched by their owner between two meetings of the cluster they took 1.5 us longer.)
-      const int per = BM / a.split;
       const uint32_t mine = smem_u32(part) + (uint32_t)((rank * 128 + tid) * per) * 4;
       __syncwarp();
       asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -314,12 +389,14 @@ f8_few_kernel(const SplitArgs a, const __grid_constant__ CUtensorMap wmap, const
       }
       __syncwarp();
       asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-      if (f_wait(joined, 0, dead, a.status) && n < a.out.n) {
-        for (int j = 0; j < per && m0 + rank * per + j < a.out.m; ++j) {
+      if (f_wait(joined, 0, dead, a.status) && on) {
+#pragma unroll
+        for (int j = 0; j < BM / 2; ++j) {
+          if (j >= per || m1 + j >= a.out.m) break;
           const float* from = part + tid * per + j;
           float v = 0.f;
           for (int q = 0; q < a.split; ++q) v += from[q * 128 * per];
-          f8_put(a.out, v, bias, m0 + rank * per + j, n);
+          f8_put(a.out, v + bias + e1[j] + e2[j], (size_t)(m1 + j) * a.out.n + n);
         }
       }
       __syncwarp();
@@ -397,12 +474,22 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
 }
 
 // Rows XR rank / SPLIT .. of the sums that the CTAs of the cluster have laid down, added in the order of the ranks, a warp to a row at a
-// time; all loads of a warp are in flight together. Tells the cluster when it has read.
-template <int XR, int SPLIT>
+// time; all loads of a warp are in flight together, the residuals' ahead of the meeting of the cluster. Tells the cluster when it has read.
+template <int XR, int SPLIT, bool RES>
 __device__ __forceinline__ void f8_join(const F8Out& o, const uint8_t* sm, int rank, int warp, int m0, int n0) {
   constexpr int PER = XR / SPLIT, ROWS = PER / 8;
-  const int lane = threadIdx.x & 31, first = rank * PER + warp;
-  float4 v[ROWS][SPLIT];
+  const int lane = threadIdx.x & 31, first = rank * PER + warp, n = n0 + 4 * lane;
+  float4 v[ROWS][SPLIT], e1[RES ? ROWS : 1], e2[RES ? ROWS : 1];
+  const float4 none = make_float4(0.f, 0.f, 0.f, 0.f), bias = o.bias ? f8_four(o.bias, n, o.n, false) : none;
+#pragma unroll
+  for (int i = 0; i < (RES ? ROWS : 0); ++i) {
+    const size_t row = (size_t)(m0 + first + 8 * i) * o.n;
+    const bool in = m0 + first + 8 * i < o.m;
+    e1[i] = in ? f8_four(o.r1 + row, n, o.n, o.vec) : none;
+    e2[i] = in && o.r2 ? f8_four(o.r2 + row, n, o.n, o.vec) : none;
+  }
+  __syncwarp();
+  cluster_sync();
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
     const int r = first + 8 * i;
@@ -411,38 +498,31 @@ __device__ __forceinline__ void f8_join(const F8Out& o, const uint8_t* sm, int r
 #pragma unroll
       for (int q = 0; q < SPLIT; ++q) v[i][q] = ld_cluster4(cluster_addr(from, (uint32_t)q));
   }
-  const int n = n0 + 4 * lane;
-  float4 bias = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (o.bias) {
-    if (n < o.n) bias.x = o.bias[n];
-    if (n + 1 < o.n) bias.y = o.bias[n + 1];
-    if (n + 2 < o.n) bias.z = o.bias[n + 2];
-    if (n + 3 < o.n) bias.w = o.bias[n + 3];
-  }
 #pragma unroll
   for (int i = 0; i < ROWS; ++i)
 #pragma unroll
-    for (int q = 1; q < SPLIT; ++q) {
-      v[i][0].x += v[i][q].x; v[i][0].y += v[i][q].y; v[i][0].z += v[i][q].z; v[i][0].w += v[i][q].w;
-    }
+    for (int q = 1; q < SPLIT; ++q) v[i][0] = f8_add(v[i][0], v[i][q]);
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
     const int m = m0 + first + 8 * i;
     if (m >= o.m) break;
+    const size_t at = (size_t)m * o.n + n;
+    float4 y = f8_add(v[i][0], bias);
+    if (RES) y = f8_add(f8_add(y, e1[RES ? i : 0]), e2[RES ? i : 0]);
     if (o.vec) {
-      if (n < o.n) f8_put4(o, v[i][0], bias, m, n);
+      if (n < o.n) f8_put4(o, y, at);
     } else {
-      const float e[4] = {v[i][0].x, v[i][0].y, v[i][0].z, v[i][0].w}, b[4] = {bias.x, bias.y, bias.z, bias.w};
+      const float e[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (n + j < o.n) f8_put(o, e[j], b[j], m, n + j);
+        if (n + j < o.n) f8_put(o, e[j], at + j);
     }
   }
 }
 
-template <int XR>
+template <int XR, bool RES>
 __global__ void __launch_bounds__(Some<XR>::THREADS, 1)
 f8_some_kernel(const SplitArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
   using F = Some<XR>;
@@ -491,6 +571,7 @@ f8_some_kernel(const SplitArgs a, const __grid_constant__ CUtensorMap wmap, cons
 #pragma unroll
     for (int i = 0; i < 32; ++i) acc[i] = make_float2(0.f, 0.f);
     pdl_wait();
+    if (RES && a.split == 1) f8_ask_residuals<64>(a.out, m0 + 32 * quad, n0 + 64 * side);
     const float* sx = a.sx + (size_t)min(m0 + 32 * quad + lane, a.out.m - 1) * a.kblocks + kb0;
     const float* sw = a.sw + (size_t)nt * a.kblocks + kb0;
     float fx = nkb ? sx[0] : 0.f, fw = nkb ? sw[0] : 0.f;
@@ -557,7 +638,7 @@ f8_some_kernel(const SplitArgs a, const __grid_constant__ CUtensorMap wmap, cons
   pdl_wait();       // for the warps that have not been in a role that waits
 
   if (a.split == 1) {
-    if (reads) f8_store_rows<64>(a.out, acc, sm + warp * TURN_BYTES, m0 + 32 * quad, n0 + 64 * side);
+    if (reads) f8_store_rows<64, RES>(a.out, acc, sm + warp * TURN_BYTES, m0 + 32 * quad, n0 + 64 * side);
   } else {
     // The sums of the cluster's ranges of K: everybody lays down its own, 512 bytes a row, 16-byte piece p of row r at place p ^ (r % 8);
     // rank q fetches rows XR q / split .. of all and adds them in the order of the ranks, a warp to a row.
@@ -567,12 +648,12 @@ f8_some_kernel(const SplitArgs a, const __grid_constant__ CUtensorMap wmap, cons
       for (int p = 0; p < 16; ++p)
         *reinterpret_cast<float4*>(sm + r * 512 + (((16 * side + p) ^ (r & 7)) << 4)) = make_float4(acc[2 * p].x, acc[2 * p].y, acc[2 * p + 1].x, acc[2 * p + 1].y);
     }
-    __syncwarp();
-    cluster_sync();
     if (warp < F::EPI_WARPS) {
-      if (a.split == 2) f8_join<XR, 2>(a.out, sm, rank, warp, m0, n0);
-      else f8_join<XR, 4>(a.out, sm, rank, warp, m0, n0);
+      if (a.split == 2) f8_join<XR, 2, RES>(a.out, sm, rank, warp, m0, n0);
+      else f8_join<XR, 4, RES>(a.out, sm, rank, warp, m0, n0);
     } else {
+      __syncwarp();
+      cluster_sync();
       asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     }
     __syncwarp();
@@ -604,7 +685,7 @@ struct PairArgs {
   int* status;
 };
 
-template <int NW>
+template <int NW, bool RES>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
   using P = Pair<NW>;
@@ -690,6 +771,7 @@ f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const
     begin(pair);
     for (int item = pair; item < items; item += npairs) {
       bool alive = true;
+      if (RES) f8_ask_residuals<HALF>(a.out, m_first, n_first);
       float2 acc[HALF / 2];
 #pragma unroll
       for (int i = 0; i < HALF / 2; ++i) acc[i] = make_float2(0.f, 0.f);
@@ -726,7 +808,7 @@ f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const
       if (!alive) break;
       const int m_done = m_first, n_done = n_first;
       if (item + npairs < items) begin(item + npairs);  // its first scales arrive meanwhile
-      f8_store_rows<HALF>(a.out, acc, turn + warp * TURN_BYTES, m_done, n_done);
+      f8_store_rows<HALF, RES>(a.out, acc, turn + warp * TURN_BYTES, m_done, n_done);
     }
   } else if (warp == PAIR_EPI_WARPS) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -843,17 +925,22 @@ int launch_few(fb200_device* dev, const F8Job& j, int split) {
   static bool configured[64] = {false};
   return launch_split(dev, j, f8_few_kernel<BM>, BM, Few<BM>::THREADS, Few<BM>::SMEM, split, configured);
 }
+template <int XR, bool RES>
+int launch_some_as(fb200_device* dev, const F8Job& j, int split) {
+  static bool configured[64] = {false};
+  return launch_split(dev, j, f8_some_kernel<XR, RES>, XR, Some<XR>::THREADS, Some<XR>::SMEM, split, configured);
+}
+// Kernels without residuals have no room set aside for them: with it 8192 rows of 28672 x 4096 took 870 us instead of 830
 template <int XR>
 int launch_some(fb200_device* dev, const F8Job& j, int split) {
-  static bool configured[64] = {false};
-  return launch_split(dev, j, f8_some_kernel<XR>, XR, Some<XR>::THREADS, Some<XR>::SMEM, split, configured);
+  return j.out.r1 ? launch_some_as<XR, true>(dev, j, split) : launch_some_as<XR, false>(dev, j, split);
 }
 
-template <int NW>
-int launch_pair(fb200_device* dev, const F8Job& j) {
+template <int NW, bool RES>
+int launch_pair_as(fb200_device* dev, const F8Job& j) {
   using P = Pair<NW>;
   static bool configured[64] = {false};
-  int rc = allow_smem(dev, f8_pair_kernel<NW>, P::SMEM, configured);
+  int rc = allow_smem(dev, f8_pair_kernel<NW, RES>, P::SMEM, configured);
   if (rc) return rc;
   CUtensorMap xmap;
   if (!fb200_make_map_2d_bytes(&xmap, j.x, j.w->k, (uint64_t)j.out.m, j.ld, 128))
@@ -865,8 +952,12 @@ int launch_pair(fb200_device* dev, const F8Job& j) {
   const long long fit = (32ll << 20) / (256ll * F8_BLOCK * j.kblocks);
   a.m_group = fit < 1 ? 1 : fit > a.m_tiles ? a.m_tiles : (int)fit;
   const int pairs = items < dev->sm_count / 2 ? (int)items : dev->sm_count / 2;
-  return fb200_launch(dev, f8_pair_kernel<NW>, dim3((unsigned)(2 * pairs)), dim3(PAIR_THREADS), (size_t)P::SMEM, true, a,
+  return fb200_launch(dev, f8_pair_kernel<NW, RES>, dim3((unsigned)(2 * pairs)), dim3(PAIR_THREADS), (size_t)P::SMEM, true, a,
                       j.w->map64, xmap);
+}
+template <int NW>
+int launch_pair(fb200_device* dev, const F8Job& j) {
+  return j.out.r1 ? launch_pair_as<NW, true>(dev, j) : launch_pair_as<NW, false>(dev, j);
 }
 
 // The kernel, by the number of rows and a small cost model in microseconds (fitted to the times below, which hold for products one after
