@@ -266,10 +266,11 @@ FB200_API int fb200_sample(fb200_device* dev, const float* logits_dev, size_t ro
  * Inputs are F32, F16 or BF16 (`type`), rows `ldx` .. elements apart; arithmetic is f32. Outputs may not overlap inputs, unless said so.
  * FB200_ERR_UNSUPPORTED_DTYPE for other types, FB200_ERR_INVALID_SHAPE for rows that overlap or are not aligned, for 2^31 rows or more
  * and for more than 2^27 columns. Zero rows or columns: nothing is written. Nothing here allocates or waits but the making of a matrix; the
- * first launch of a kernel sets it up and loads its code, so make a call of the same sizes before a stream capture. */
+ * first launch of a kernel sets it up and loads its code, so make a call of the same sizes, types and epilogue before a stream capture. */
 FB200_API int fb200_quantize_f8(fb200_device* dev, const void* x_dev, size_t ldx, uint32_t type, size_t rows, size_t n, uint8_t* codes_dev,
                                 size_t ld, float* scales_dev);
-/* The same of silu(gate) * up, the hidden row of a gated feed-forward (gate and up may be halves of the same rows). */
+/* The same of silu(gate) * up, the hidden row of a gated feed-forward (gate and up may be halves of the same rows). A gate below -87
+ * counts as one whose silu is 0. */
 FB200_API int fb200_silu_mul_f8(fb200_device* dev, const void* gate_dev, size_t ldgate, const void* up_dev, size_t ldup, uint32_t type,
                                 size_t rows, size_t n, uint8_t* codes_dev, size_t ld, float* scales_dev);
 /* The same of an RMSNorm: s = x (+ residual), v = s / sqrt(mean(s^2) + eps) * weight (+ bias), weight and bias f32 [n]. residual_dev,

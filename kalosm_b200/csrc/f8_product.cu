@@ -167,7 +167,7 @@ __device__ __forceinline__ void f8_store_rows(const F8Out& o, const float2 (&acc
     return;
   }
   // o.vec: a lane has four columns of every fourth row. The residuals of four rows are in flight together, all loads ahead of the stores (y
-  // may be a residual, so that the compiler moves none): 8192 rows of 4096 x 4096 to f32 with one take 165 us, 4000 rows of 5000 x 700 take
+  // may be a residual, so that the compiler moves none): 8192 rows of 4096 x 4096 to f32 with one take 171 us, 4000 rows of 5000 x 700 take
   // 57, one row at a time 125. Eight rows at a time spilled registers: 197 and 75 us.
   const int n4 = n0 + 4 * (lane & 7);
   const size_t at4 = (size_t)(m0 + (lane >> 3)) * o.n + n4;

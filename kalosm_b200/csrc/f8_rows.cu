@@ -125,7 +125,7 @@ __device__ __forceinline__ void f8_emit(const float (&v)[E], uint32_t top, int c
 }
 
 // silu(g) u = g u / (1 + exp(-g)), with the fast exponential (2 + 1.2 |g| units of its last place) and quotient (2 units): a code keeps
-// four bits
+// four bits. Divisors above 2^126 (g below -87.3) give 0.
 __device__ __forceinline__ float f8_silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
 // Blocks by themselves: a warp takes STEPS x 32 x PER_LANE columns of a row, `wpr` warps stand side by side in a row. Its pieces
@@ -226,8 +226,8 @@ struct NormArgs {
 };
 
 // A row per CTA at a time, kept in registers between its sum of squares and its norm: CHUNKS pieces a thread. AHEAD: the CTA's next row is
-// asked for before this one's sum is complete, and the weight stays in registers from row to row. The sum of squares and the norm are of the unrounded sum x + residual; sum_dev gets it
-// rounded to the type of x, once.
+// asked for before this one's sum is complete, and with one piece a thread the weight stays in registers from row to row. The sum of
+// squares and the norm are of the unrounded sum x + residual; sum_dev gets it rounded to the type of x, once.
 template <typename T, int CHUNKS, bool AHEAD>
 __global__ void __launch_bounds__(1024)
 rms_norm_f8_kernel(const NormArgs<T> a, size_t rows) {

@@ -341,6 +341,26 @@ def test_product_over_borrowed_codes_and_into_its_residual(dev):
         check("f32", stream.as_slice(), y + r, bound + F.U * (np.abs(y) + bound + np.abs(r)))
 
 
+@pytest.mark.parametrize("tile,m", [("16,1", 40), ("32,4", 45), ("64,1", 75), ("128,1", 155), ("128,4", 155), ("pair,128", 301), ("pair,256", 301)])
+@pytest.mark.parametrize("n", [516, 389])
+@pytest.mark.parametrize("second", [False, True])
+def test_product_into_either_residual(dev, monkeypatch, tile, m, n, second):
+    """y takes the place of r1 or of r2 while both are added: every residual is read before its place is written."""
+    monkeypatch.setenv("FB200_F8_TILE", tile)
+    rng = np.random.default_rng(n + m)
+    x, xs, w, ws = operands(rng, m, n, 700)
+    y, bound = F.product(x, xs, w, ws)
+    a, b = (rng.standard_normal((m, n)).astype(np.float32) for _ in range(2))
+    for r in (a, b):
+        bound = bound + F.U * (np.abs(y) + bound + np.abs(r))
+        y = y + r
+    r1, r2 = dev.tensor(a), dev.tensor(b)
+    out = r2 if second else r1
+    device_rows(dev, x, xs).f8_mat_mul(kb.F8Matrix.from_raw_bytes(dev, (n, 700), w, ws), epilogue=kb.EPI_RESIDUAL, r1=r1, r2=r2, out=out)
+    check("f32", out.as_slice(), y, bound)
+    assert np.array_equal((r1 if second else r2).as_slice(), a if second else b)
+
+
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("tile,m", [("16,2", 9), ("64,2", 40), ("128,1", 140), ("pair,256", 300)])
 def test_product_into_unaligned_rows(dev, monkeypatch, kind, tile, m):
