@@ -14,7 +14,7 @@
 //  * f8_some_kernel, to a few hundred: 64 or 128 activation rows (in the M role, so that a thread has one row and one scale) by 128 weight
 //    rows, K split over clusters of up to four. Bound: HBM, then what an SM takes in from L2 (94 GB/s measured). 128 rows of
 //    4096 x 14336: 16.4 us (3.7 TB/s, 0.92 PFLOP/s);
-//  * f8_pair_kernel: CTA pairs, 256 activation rows by 128 or 256 weight rows, persistent. Bound: what the SMs take in from L2 (32 KB per pair
+//  * f8_pair_kernel: CTA pairs, 256 activation rows by 128, 192 or 256 weight rows, persistent. Bound: what the SMs take in from L2 (32 KB per pair
 //    tile and block and SM: without its MMAs the kernel takes 0.9 of its time) and the power limit. 8192 rows of 28672 x 4096: 831 us
 //    (2.3 PFLOP/s), 930 us at the 1.4 GHz that 950 W leave in a long run.
 // Every wait is bounded (2^22 polls): one that gives up sets the device status word and a flag that makes the other roles leave; copies
@@ -34,7 +34,7 @@ struct fb200_f8matrix {
   uint8_t* codes = nullptr;
   float* scales = nullptr;
   bool owned = false;
-  CUtensorMap map128, map64;  // boxes of 128 and of 64 rows
+  CUtensorMap map128, map64, map48;  // boxes of 128, 64 and 48 rows
 };
 
 namespace {
@@ -148,11 +148,12 @@ __device__ __forceinline__ void f8_store_rows(const F8Out& o, const float2 (&acc
   if (!RES && o.pack) {
     uint16_t* to = reinterpret_cast<uint16_t*>(o.y) + (size_t)m0 * o.n + n0 + 8 * (lane & 7);
 #pragma unroll
-    for (int c = 0; c < COLS / 64; ++c) {
+    for (int c = 0; c < (COLS + 63) / 64; ++c) {
       if (64 * c >= n_end) break;
+      const int pieces = COLS - 64 * c < 64 ? (COLS - 64 * c) / 8 : 8;
       __syncwarp();
 #pragma unroll
-      for (int p = 0; p < 8; ++p) {
+      for (int p = 0; p < pieces; ++p) {
         const float2* v = acc + 32 * c + 4 * p;
         mine[p ^ (lane & 7)] = make_uint4(f8_pair(o, v[0]), f8_pair(o, v[1]), f8_pair(o, v[2]), f8_pair(o, v[3]));
       }
@@ -161,7 +162,7 @@ __device__ __forceinline__ void f8_store_rows(const F8Out& o, const float2 (&acc
       for (int i = 0; i < 8; ++i) {
         const int r = 4 * i + (lane >> 3);
         const uint4 v = *reinterpret_cast<const uint4*>(turn + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-        if (r < rows && 64 * c + 8 * (lane & 7) < n_end) *reinterpret_cast<uint4*>(to + (size_t)r * o.n + 64 * c) = v;
+        if (r < rows && 64 * c + 8 * (lane & 7) < n_end && (pieces == 8 || (lane & 7) < pieces)) *reinterpret_cast<uint4*>(to + (size_t)r * o.n + 64 * c) = v;
       }
     }
     return;
@@ -671,11 +672,13 @@ f8_some_kernel(const SplitArgs a, const __grid_constant__ CUtensorMap wmap, cons
 constexpr int PAIR_EPI_WARPS = 8, PAIR_THREADS = (PAIR_EPI_WARPS + 4) * 32, PAIR_MAX_STAGES = 8;
 template <int NW>
 struct Pair {
-  static constexpr int STAGE = F8_A_BYTES + NW / 2 * 128, STAGES = NW == 256 ? 6 : 8, TMEM = 512;
-  static constexpr int PARTS = NW / 128, BUFS = 4 / PARTS;  // four accumulators of 128 columns: PARTS of a block of K, BUFS blocks
+  static constexpr int STAGE = F8_A_BYTES + NW / 2 * 128, STAGES = NW == 128 ? 8 : 6, TMEM = 512;
+  // four accumulators of WIDE columns, 128 columns apart: PARTS of a block of K, BUFS blocks
+  static constexpr int PARTS = NW > 128 ? 2 : 1, BUFS = 4 / PARTS, WIDE = NW / PARTS;
   static constexpr int SMEM = STAGES * STAGE + PAIR_EPI_WARPS * TURN_BYTES + 256 + 1024;
-  // instruction descriptor: f32 accumulator, e4m3 A and B, both K-major, N = 128, M = 256 over the pair
-  static constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+  static_assert(PARTS == 2 || STAGES % 2 == 0, "a stage belongs to one issuer");
+  // instruction descriptor: f32 accumulator, e4m3 A and B, both K-major, N = WIDE, M = 256 over the pair
+  static constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(WIDE >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
 };
 
 struct PairArgs {
@@ -726,11 +729,12 @@ f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const
     mt = first + at - nt * height;
   };
   const int pre = min(P::STAGES, a.kblocks);
-  // of every 128 columns of a product a CTA holds 64 weight rows
+  // a CTA holds one half of the weight rows of every part
   auto weights = [&](int s, int kb, int nt) {
 #pragma unroll
     for (int p = 0; p < P::PARTS; ++p)
-      pair_tma_box2(smem_u32(sm + s * P::STAGE) + F8_A_BYTES + p * 64 * 128, &wmap, kb * F8_BLOCK, nt * NW + 128 * p + rank * 64, cluster_addr(full + 8 * s, 0));
+      pair_tma_box2(smem_u32(sm + s * P::STAGE) + F8_A_BYTES + p * (P::WIDE / 2 * 128), &wmap, kb * F8_BLOCK, nt * NW + P::WIDE * p + rank * (P::WIDE / 2),
+                    cluster_addr(full + 8 * s, 0));
   };
   if (tid == PAIR_EPI_WARPS * 32) {
     int mt, nt;
@@ -757,6 +761,11 @@ f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const
     int m_first = 0, n_first = 0;
     const float *sx = nullptr, *sw = nullptr;
     float fx = 0.f, fw = 0.f;  // scales of the next block
+    // 96 columns may be of two scales, columns 32 `turns` .. of the second
+    constexpr bool TWO = HALF % 64 != 0;
+    const float* sw2 = nullptr;
+    float fw2 = 0.f;
+    int turns = 0;
     auto begin = [&](int item) {
       int mt, nt;
       split(item, mt, nt);
@@ -766,6 +775,11 @@ f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const
       sw = a.sw + (size_t)min(n_first / F8_BLOCK, (a.out.n - 1) / F8_BLOCK) * a.kblocks;
       fx = sx[0];
       fw = sw[0];
+      if (TWO) {
+        turns = (F8_BLOCK - n_first % F8_BLOCK) / 32;
+        sw2 = a.sw + (size_t)min((n_first + HALF - 1) / F8_BLOCK, (a.out.n - 1) / F8_BLOCK) * a.kblocks;
+        fw2 = sw2[0];
+      }
     };
     pdl_wait();
     begin(pair);
@@ -781,9 +795,10 @@ f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const
         if (!(alive = f_wait(acc_full + 8 * buf, k / P::BUFS & 1, dead, a.status))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t tl = tmem + ((uint32_t)(32 * quad) << 16) + buf * 128 + (P::PARTS == 2 ? 0 : side * HALF);
-        const float2 f = make_float2(fx * fw, fx * fw);
+        const float2 f = make_float2(fx * fw, fx * fw), f2 = make_float2(fx * fw2, fx * fw2);
         fx = sx[min(kb + 1, a.kblocks - 1)];  // in flight until the next block
         fw = sw[min(kb + 1, a.kblocks - 1)];
+        if (TWO) fw2 = sw2[min(kb + 1, a.kblocks - 1)];
         uint32_t v[4][16];
         x_ld16(tl, v[0]);
         x_ld16(tl + 16, v[1]);
@@ -801,7 +816,7 @@ f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const uint32_t* p = &v[(2 * c & 3) + i / 8][2 * i % 16];
-            acc[16 * c + i] = fma2(make_float2(__uint_as_float(p[0]), __uint_as_float(p[1])), f, acc[16 * c + i]);
+            acc[16 * c + i] = fma2(make_float2(__uint_as_float(p[0]), __uint_as_float(p[1])), TWO && c >= turns ? f2 : f, acc[16 * c + i]);
           }
         }
       }
@@ -841,13 +856,14 @@ f8_pair_kernel(const PairArgs a, const __grid_constant__ CUtensorMap wmap, const
     }
   } else if (warp <= PAIR_EPI_WARPS + 2) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    // ---- two MMA issuers (even CTA), an accumulator of 128 weight rows and a block of K at a time: of the two parts of a block one each,
-    // or every other block. (One warp needs 460 cycles for an accumulator's waits, MMAs and commits, nearly twice what the MMAs take.)
+    // ---- two MMA issuers (even CTA), an accumulator of WIDE weight rows and a block of K at a time: of the two parts of a block one each,
+    // or every other block. (One warp needs 460 cycles for an accumulator's waits, MMAs and commits, nearly twice what the MMAs take. One
+    // accumulator of all NW columns, every other block each: the same time with 256, 2 % more with 192.)
     const uint32_t which = warp - PAIR_EPI_WARPS - 1, part = P::PARTS == 2 ? which : 0, step = 2 / P::PARTS;
     const uint32_t blocks = (uint32_t)((items - pair + npairs - 1) / npairs) * (uint32_t)a.kblocks;
     if (rank == 0) {
       pdl_wait();
-      const uint64_t adesc0 = x_desc_rows(smem_u32(sm)), bdesc0 = x_desc_rows(smem_u32(sm) + F8_A_BYTES) + part * (64 * 128 >> 4);
+      const uint64_t adesc0 = x_desc_rows(smem_u32(sm)), bdesc0 = x_desc_rows(smem_u32(sm) + F8_A_BYTES) + part * (P::WIDE / 2 * 128 >> 4);
       uint32_t s = P::PARTS == 2 ? 0 : which, parity = 0;
       for (uint32_t k = s; k < blocks; k += step) {
         const uint32_t buf = k % P::BUFS * P::PARTS + part;
@@ -953,7 +969,7 @@ int launch_pair_as(fb200_device* dev, const F8Job& j) {
   a.m_group = fit < 1 ? 1 : fit > a.m_tiles ? a.m_tiles : (int)fit;
   const int pairs = items < dev->sm_count / 2 ? (int)items : dev->sm_count / 2;
   return fb200_launch(dev, f8_pair_kernel<NW, RES>, dim3((unsigned)(2 * pairs)), dim3(PAIR_THREADS), (size_t)P::SMEM, true, a,
-                      j.w->map64, xmap);
+                      NW == 192 ? j.w->map48 : j.w->map64, xmap);
 }
 template <int NW>
 int launch_pair(fb200_device* dev, const F8Job& j) {
@@ -967,8 +983,9 @@ int launch_pair(fb200_device* dev, const F8Job& j) {
 //    4096 x 14336: 12.3, with the kernel for some rows 14.3;
 //  * above, single CTAs with 64 or 128 rows: a round takes 0.28 or 0.31 a block and 3 more, a split 2 more. By 8 it was slower (16 clusters of
 //    8 do not run at once: 64 rows of 4096 x 4096 8.6 us by 4, 17.8 by 8);
-//  * against pairs: a round takes 0.27 (128 weight rows) or 0.42 (256) a block and 1.5 more, 3.5 around them. 512 rows of 4096 x 4096: 13.6 us
-//    on single CTAs, 14.3 on pairs; 1024 of 6144 x 4096: 38.2 on single CTAs, 33.4 on pairs of 256, 35.1 of 128.
+//  * against pairs: a round takes 0.27 (128 weight rows), 0.39 (192) or 0.42 (256) a block and 1.5 more, 3.5 around them. 512 rows of
+//    4096 x 4096: 13.6 us on single CTAs, 14.3 on pairs; 1024 of 6144 x 4096: 38.2 on single CTAs, 35.3, 31.5 and 34.0 on pairs of 128, 192
+//    and 256 (three, two and two rounds); 4096 of 6144 x 4096, where 256 take a round less: 125.6, 105.7 and 99.8.
 int f8_product(fb200_device* dev, const F8Job& j) {
   const int m = j.out.m, n_tiles = (j.out.n + 127) / 128;
   int rows = m <= 16 ? 16 : 32, split = 1, pair = 0;
@@ -983,25 +1000,25 @@ int f8_product(fb200_device* dev, const F8Job& j) {
         const double cost = (double)((tiles + room - 1) / room) * ((j.kblocks + c - 1) / c * (r == 64 ? 0.28 : 0.31) + 3.0) + (c > 1 ? 2.0 : 0.0);
         if (cost < best) best = cost, rows = r, split = c;
       }
-    for (int nw = 128; nw <= 256; nw *= 2) {
+    for (int nw = 128; nw <= 256; nw += 64) {
       const long long items = (long long)((j.out.n + nw - 1) / nw) * ((m + 255) / 256);
       const int room = dev->sm_count / 2;
-      const double cost = (double)((items + room - 1) / room) * (j.kblocks * (nw == 128 ? 0.27 : 0.42) + 1.5) + 3.5;
+      const double cost = (double)((items + room - 1) / room) * (j.kblocks * (nw == 128 ? 0.27 : nw == 192 ? 0.39 : 0.42) + 1.5) + 3.5;
       if (cost < best) best = cost, pair = nw;
     }
   }
   // FB200_F8_TILE (tests, tuning; read per call): "ROWS,SPLIT" activation rows (16, 32, 64, 128) and ranges of K (8 with 16 or 32 rows
-  // only) of the kernels on single CTAs, "pair,NW" pairs with 128 or 256 weight rows; what there is not leaves the choice to the rule
+  // only) of the kernels on single CTAs, "pair,NW" pairs with 128, 192 or 256 weight rows; what there is not leaves the choice to the rule
   if (const char* cfg = getenv("FB200_F8_TILE")) {
     int frows, fsplit;
     if (sscanf(cfg, "pair,%d", &frows) == 1) {
-      if (frows == 128 || frows == 256) pair = frows;
+      if (frows == 128 || frows == 192 || frows == 256) pair = frows;
     } else if (sscanf(cfg, "%d,%d", &frows, &fsplit) == 2 && (frows == 16 || frows == 32 || frows == 64 || frows == 128) &&
                (fsplit == 1 || fsplit == 2 || fsplit == 4 || (fsplit == 8 && frows <= 32))) {
       rows = frows, split = fsplit, pair = 0;
     }
   }
-  if (pair) return pair == 128 ? launch_pair<128>(dev, j) : launch_pair<256>(dev, j);
+  if (pair) return pair == 128 ? launch_pair<128>(dev, j) : pair == 192 ? launch_pair<192>(dev, j) : launch_pair<256>(dev, j);
   switch (rows) {
     case 16: return launch_few<16>(dev, j, split);
     case 32: return launch_few<32>(dev, j, split);
@@ -1018,7 +1035,8 @@ int check_shape(fb200_device* dev, const char* op, const uint64_t* shape, int ra
 }
 
 int make_maps(fb200_device* dev, fb200_f8matrix* w) {
-  if (fb200_make_map_2d_bytes(&w->map128, w->codes, w->k, w->n, w->ld, 128) && fb200_make_map_2d_bytes(&w->map64, w->codes, w->k, w->n, w->ld, 64))
+  if (fb200_make_map_2d_bytes(&w->map128, w->codes, w->k, w->n, w->ld, 128) && fb200_make_map_2d_bytes(&w->map64, w->codes, w->k, w->n, w->ld, 64) &&
+      fb200_make_map_2d_bytes(&w->map48, w->codes, w->k, w->n, w->ld, 48))
     return FB200_OK;
   return fb200_fail(dev, FB200_ERR_CUDA, "F8Matrix: tensor map refused (%llu x %llu)", (unsigned long long)w->n, (unsigned long long)w->k);
 }

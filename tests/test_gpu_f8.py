@@ -219,7 +219,7 @@ def test_rms_norm_of_zero_and_not_finite_rows(dev):
 
 # ---- the product --------------------------------------------------------------------------------------------------------
 
-TILES = ["16,1", "16,2", "16,4", "16,8", "32,1", "32,4", "32,8", "64,1", "64,2", "64,4", "128,1", "128,2", "128,4", "pair,128", "pair,256"]
+TILES = ["16,1", "16,2", "16,4", "16,8", "32,1", "32,4", "32,8", "64,1", "64,2", "64,4", "128,1", "128,2", "128,4", "pair,128", "pair,192", "pair,256"]
 
 
 def operands(rng, m, n, k):
@@ -278,7 +278,7 @@ def test_product_tiles(dev, monkeypatch, tile, m, n, k):
 @pytest.mark.parametrize("m,n,k", [(300, 256 * 40, 300), (300, 256 * 40 - 77, 1000), (256, 256 * 75, 128), (513, 256 * 50 + 3, 130), (256, 256 * 111, 900)])
 def test_product_several_tiles_per_pair(dev, monkeypatch, m, n, k):
     """More tiles than pairs, so that a pair goes from tile to tile (148 SMs: 80, 80, 75, 153 and 111 tiles of 256 x 256 on 74 pairs)."""
-    for tile in ("pair,256", "pair,128"):
+    for tile in ("pair,256", "pair,192", "pair,128"):
         monkeypatch.setenv("FB200_F8_TILE", tile)
         run_product(dev, np.random.default_rng(n), m, n, k, "bf16")
     run_product(dev, np.random.default_rng(n), m, n, k, "f32", kb.EPI_BIAS)
@@ -292,7 +292,7 @@ def test_product_rows(dev, m, n, k):
 
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("epilogue,second", [(kb.EPI_NONE, False), (kb.EPI_RESIDUAL, False), (kb.EPI_RESIDUAL, True), (kb.EPI_BIAS, False)])
-@pytest.mark.parametrize("tile,m", [("16,2", 5), ("64,1", 60), ("128,4", 300), ("pair,128", 300), ("pair,256", 300)])
+@pytest.mark.parametrize("tile,m", [("16,2", 5), ("64,1", 60), ("128,4", 300), ("pair,128", 300), ("pair,192", 300), ("pair,256", 300)])
 @pytest.mark.parametrize("n", [260, 333])
 def test_product_epilogues(dev, monkeypatch, kind, epilogue, second, tile, m, n):
     monkeypatch.setenv("FB200_F8_TILE", tile)
@@ -305,7 +305,7 @@ def test_product_model_sizes(dev, m, n, k):
     run_product(dev, np.random.default_rng(k), m, n, k, "bf16", kb.EPI_RESIDUAL)
 
 
-@pytest.mark.parametrize("tile,m", [("16,4", 9), ("64,2", 50), ("128,2", 260), ("pair,128", 260), ("pair,256", 260)])
+@pytest.mark.parametrize("tile,m", [("16,4", 9), ("64,2", 50), ("128,2", 260), ("pair,128", 260), ("pair,192", 260), ("pair,256", 260)])
 def test_product_is_repeatable(dev, monkeypatch, tile, m):
     monkeypatch.setenv("FB200_F8_TILE", tile)
     x, xs, w, ws = operands(np.random.default_rng(m), m, 1300, 2000)
@@ -315,7 +315,7 @@ def test_product_is_repeatable(dev, monkeypatch, tile, m):
         assert np.array_equal(rows.f8_mat_mul(mat).as_slice(), first)
 
 
-@pytest.mark.parametrize("tile,m", [("16,2", 9), ("128,2", 260), ("pair,128", 260), ("pair,256", 260)])
+@pytest.mark.parametrize("tile,m", [("16,2", 9), ("128,2", 260), ("pair,128", 260), ("pair,192", 260), ("pair,256", 260)])
 def test_product_keeps_what_is_not_finite_in_its_row_and_column(dev, monkeypatch, tile, m):
     monkeypatch.setenv("FB200_F8_TILE", tile)
     x, xs, w, ws = operands(np.random.default_rng(m), m, 400, 600)
@@ -341,7 +341,7 @@ def test_product_over_borrowed_codes_and_into_its_residual(dev):
         check("f32", stream.as_slice(), y + r, bound + F.U * (np.abs(y) + bound + np.abs(r)))
 
 
-@pytest.mark.parametrize("tile,m", [("16,1", 40), ("32,4", 45), ("64,1", 75), ("128,1", 155), ("128,4", 155), ("pair,128", 301), ("pair,256", 301)])
+@pytest.mark.parametrize("tile,m", [("16,1", 40), ("32,4", 45), ("64,1", 75), ("128,1", 155), ("128,4", 155), ("pair,128", 301), ("pair,192", 301), ("pair,256", 301)])
 @pytest.mark.parametrize("n", [516, 389])
 @pytest.mark.parametrize("second", [False, True])
 def test_product_into_either_residual(dev, monkeypatch, tile, m, n, second):
@@ -362,7 +362,7 @@ def test_product_into_either_residual(dev, monkeypatch, tile, m, n, second):
 
 
 @pytest.mark.parametrize("kind", TYPES)
-@pytest.mark.parametrize("tile,m", [("16,2", 9), ("64,2", 40), ("128,1", 140), ("pair,256", 300)])
+@pytest.mark.parametrize("tile,m", [("16,2", 9), ("64,2", 40), ("128,1", 140), ("pair,192", 300), ("pair,256", 300)])
 def test_product_into_unaligned_rows(dev, monkeypatch, kind, tile, m):
     """Outputs and residuals one element behind an aligned address, in a width that would allow wide stores."""
     monkeypatch.setenv("FB200_F8_TILE", tile)
